@@ -187,8 +187,11 @@ def prepare(case, seed):
         B, T, V, C = (case[k] for k in ("B", "T", "V", "C"))
         s["table"] = normal(V, C, scale=0.02)
         s["positions"] = normal(T, C, scale=0.01) if case["positions"] else None
-        rank = torch.arange(1, V + 1, device=dev, dtype=torch.float32) ** -case["zipf"]
-        pick = torch.multinomial(rank, B * T, replacement=True, generator=g)
+        # ranks with a share proportional to rank ** -zipf, by the inverse of their distribution
+        # (element by element: a running sum of the shares rounds differently from run to run)
+        u, z = torch.rand(B * T, generator=g, device=dev, dtype=torch.float64), 1.0 - case["zipf"]
+        rank = (u * math.log(V)).exp() if z == 0 else (1 + u * (V**z - 1)) ** (1 / z)
+        pick = (rank.long() - 1).clamp(0, V - 1)
         s["tokens"] = torch.randperm(V, generator=g, device=dev)[pick].view(B, T)
         s["padding"] = None
         if case["padding"]:  # sequences end in padding

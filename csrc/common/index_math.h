@@ -93,6 +93,17 @@ NF_IX int mfma32_acc_row(int reg, int lane) {
     return (reg & 3) + 8 * (reg >> 2) + 4 * (lane >> 5);
 }
 
+// ---- attention tiles (attention_general.hip) -----------------------------------------
+// byte offset of 16-byte piece `piece` of row `row` in a tile of `width` (64 or 128) 16-bit
+// columns.  The pieces of a row are permuted so that both kinds of reads cover all 16 slots of
+// the 256-byte bank row: the 16 rows of a ds_read_b128 group at one piece, and the four
+// consecutive rows at four consecutive pieces that 32 lanes of a transposing read take.
+NF_IX int attn_off(int width, int row, int piece) {
+    const int x = width == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3)
+                              : ((row & 3) << 2) | ((row >> 2) & 3);
+    return row * width * 2 + ((piece ^ x) << 4);
+}
+
 // ---- 3x3 convolution tiles (conv_ops.hip) ---------------------------------------------
 // A tile is NI bands of RI image rows; its LDS patch holds, per band, RI + 2 rows of
 // W + 2 pixels (the halo).  H, W, RI are powers of two.

@@ -57,6 +57,29 @@ NF_HD Philox4 philox4x32_10(uint64_t seed, uint64_t offset, uint64_t block) {
     return Philox4{{c0, c1, c2, c3}};
 }
 
+// The generator of the dropout masks: seven rounds, the counter given as its four words.
+// (Seven is the number of rounds from which Philox4x32 passes the BigCrush battery - Salmon,
+// Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011 -; a mask inside
+// attention costs about as much as the softmax it masks, so the three further rounds of the
+// noise generator above are not taken there.)
+NF_HD Philox4 philox4x32_7(uint64_t seed, uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
+    const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u;
+    const uint32_t W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
+    uint32_t k0 = static_cast<uint32_t>(seed);
+    uint32_t k1 = static_cast<uint32_t>(seed >> 32);
+#if defined(__HIPCC__)
+#pragma unroll
+#endif
+    for (int r = 0; r < 7; ++r) {
+        const uint64_t p0 = static_cast<uint64_t>(M0) * c0, p1 = static_cast<uint64_t>(M1) * c2;
+        const uint32_t n0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
+        const uint32_t n2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
+        c0 = n0; c1 = static_cast<uint32_t>(p1); c2 = n2; c3 = static_cast<uint32_t>(p0);
+        k0 += W0; k1 += W1;
+    }
+    return Philox4{{c0, c1, c2, c3}};
+}
+
 NF_HD float u01(uint32_t x) { return static_cast<float>(x >> 8) * 5.9604644775390625e-8f; }
 NF_HD float u01_open_low(uint32_t x) {
     return (static_cast<float>(x >> 8) + 1.0f) * 5.9604644775390625e-8f;

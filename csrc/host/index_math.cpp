@@ -14,6 +14,7 @@ int nf_ix_mnist_fwd_off(int row, int col, int chunk) { return nfix::mnist_fwd_of
 int nf_ix_mnist_fwd_block_dy(int m) { return nfix::mnist_fwd_block_dy(m); }
 int nf_ix_mnist_fwd_block_dx(int m) { return nfix::mnist_fwd_block_dx(m); }
 int nf_ix_mnist_dg_off(int pr, int pc, int part) { return nfix::mnist_dg_off(pr, pc, part); }
+int nf_ix_attn_off(int width, int row, int piece) { return nfix::attn_off(width, row, piece); }
 int nf_ix_lds_b128_group(int lane) { return nfix::lds_b128_group(lane); }
 int nf_ix_mfma32_acc_row(int reg, int lane) { return nfix::mfma32_acc_row(reg, lane); }
 int nf_ix_conv_patch_source(int H, int W, int logH, int RI, int Cin, int row0, int pp) {

@@ -1,5 +1,12 @@
-"""Causal self-attention on the packed ``[B*T, 3C]`` q|k|v layout
-(csrc/hip/attention.hip: MFMA flash attention, head dimension 64).
+"""Attention for the GPT-2 configuration.
+
+``causal_attention_fwd`` / ``_bwd``: causal self-attention on the packed ``[B*T, 3C]`` q|k|v layout
+(csrc/hip/attention.hip: MFMA flash attention, head dimension 64, lengths that are multiples of 128).
+
+``attention_fwd`` / ``attention_bwd`` (csrc/hip/attention_general.hip): any length from one token
+on, strided ``[B, T, H, D]`` operands, shared key heads, head dimensions up to 128, a length per
+sequence, and dropped probabilities whose mask is a function of (seed, step, place) and never
+stored.
 
 Device tensors run the gfx950 kernels; CPU tensors run PyTorch's
 ``scaled_dot_product_attention`` in fp32 (and autograd for the backward),
@@ -9,7 +16,7 @@ layer; this serves the GPT-2 configuration of the benchmark suite.
 
 from __future__ import annotations
 
-from ctypes import c_int, c_void_p
+from ctypes import Structure, byref, c_float, c_int, c_long, c_uint, c_ulong, c_void_p
 
 import torch
 import torch.nn.functional as F
@@ -17,6 +24,7 @@ import torch.nn.functional as F
 from nanofed_amd.core.exceptions import DeviceError
 
 from . import library
+from .dropout import check_key, limit_of, philox_words
 
 P, I = c_void_p, c_int
 _SIGS = {
@@ -24,6 +32,8 @@ _SIGS = {
     "nf_attn_fwd": ([P, P, P, I, I, I, P], I),
     "nf_attn_bwd": ([P, P, P, P, P, P, I, I, I, P], I),
     "nf_attn_set_split": ([I], None),
+    "nf_attention_args_size": ([], I),
+    "nf_attention": ([P, I, I, P], I),
 }
 _fns: dict[str, object] = {}
 HEAD_DIM = 64
@@ -112,3 +122,229 @@ def causal_attention_bwd(qkv: torch.Tensor, out: torch.Tensor, lse: torch.Tensor
         y = y.transpose(1, 2).reshape(batch * seq, C)
         (g,) = torch.autograd.grad(y, leaf, dout.float())
     dqkv.copy_(g.to(torch.bfloat16))
+
+
+# ---------------------------------------------------------------------------
+# any length, layout and head grouping
+
+MAX_HEAD_DIM = 128
+_TYPES = {torch.bfloat16: 1, torch.float16: 2}
+
+
+class _Strides(Structure):
+    _fields_ = [("b", c_long), ("t", c_long), ("h", c_long)]
+
+
+class _Args(Structure):
+    """Mirror of ``AttnArgs`` in csrc/hip/attention_general.hip."""
+
+    _fields_ = [
+        ("q", P), ("k", P), ("v", P), ("out", P), ("lse", P), ("dout", P), ("dq", P), ("dk", P),
+        ("dv", P), ("delta", P), ("qlen", P), ("klen", P), ("step_at", P),
+        ("s_q", _Strides), ("s_k", _Strides), ("s_v", _Strides), ("s_out", _Strides),
+        ("s_dout", _Strides), ("s_dq", _Strides), ("s_dk", _Strides), ("s_dv", _Strides),
+        ("seed", c_ulong), ("first_head", c_ulong),
+        ("B", I), ("Tq", I), ("Tk", I), ("H", I), ("Hk", I), ("D", I), ("causal", I),
+        ("scale", c_float), ("up", c_float), ("limit", c_uint), ("step", c_uint),
+    ]
+
+
+def _operand(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, written: bool) -> _Strides:
+    """Checks a ``[B, T, heads, D]`` operand; its distances between sequences, rows and heads."""
+    if t.dtype != like.dtype or t.device != like.device:
+        raise DeviceError(f"attention: {name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape:
+        raise DeviceError(f"attention: {name} must be {list(shape)}, got {list(t.shape)}")
+    strides = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+    if shape[3] > 1 and strides[3] != 1:
+        raise DeviceError(f"attention: the columns of {name} must be contiguous")
+    if t.device.type == "cuda" and (t.data_ptr() % 16 or any(s % 8 for s in strides[:3])):
+        raise DeviceError(f"attention: rows of {name} must start at multiples of 16 bytes")
+    if written and any(n > 1 and s == 0 for n, s in zip(t.shape, strides)):
+        raise DeviceError(f"attention: {name} is written and must not be expanded")
+    return _Strides(*strides[:3])
+
+
+def _lengths(t: torch.Tensor | None, name: str, like: torch.Tensor) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.shape != like.shape[:1] or t.device != like.device:
+        raise DeviceError(f"attention: {name} must be {like.shape[0]} contiguous int32 on {like.device}")
+    return t.data_ptr()
+
+
+def _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch) -> _Args:
+    if q.dim() != 4 or k.dim() != 4:
+        raise DeviceError("attention: q, k and v are [batch, length, heads, head dimension]")
+    if q.dtype not in _TYPES and not (q.device.type == "cpu" and q.dtype in (torch.float32, torch.float64)):
+        raise DeviceError(f"attention: bfloat16 or float16, got {q.dtype}")
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    if Hk == 0 or H % Hk:
+        raise DeviceError(f"attention: {H} query heads do not share {Hk} key heads evenly")
+    if not 0 < D <= MAX_HEAD_DIM or D % 8:
+        raise DeviceError(f"attention: the head dimension must be a multiple of 8 up to {MAX_HEAD_DIM}, got {D}")
+    if max(Tq, Tk) > 1 << 22 or B * H > 1 << 23:
+        raise DeviceError("attention: lengths go up to 2^22, batch * heads up to 2^23")
+    scale = D**-0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise DeviceError("attention: the scale must be positive")
+    limit = limit_of(dropout, 8, "attention")
+    check_key(seed, step, q.device, "attention")
+    if first_batch < 0:
+        raise DeviceError("attention: first_batch must not be negative")
+    a = _Args(B=B, Tq=Tq, Tk=Tk, H=H, Hk=Hk, D=D, causal=bool(causal), scale=scale, limit=limit,
+              up=256 / (256 - limit), seed=seed, first_head=first_batch * H)
+    for name, t, shape in (("q", q, (B, Tq, H, D)), ("k", k, (B, Tk, Hk, D)), ("v", v, (B, Tk, Hk, D))):
+        setattr(a, "s_" + name, _operand(t, name, shape, q, False))
+        setattr(a, name, t.data_ptr())
+    a.qlen, a.klen = _lengths(q_lengths, "q_lengths", q), _lengths(k_lengths, "k_lengths", q)
+    if isinstance(step, torch.Tensor):
+        a.step_at = step.data_ptr()
+    else:
+        a.step = step
+    return a
+
+
+def _add(a: _Args, q: torch.Tensor, **operands: torch.Tensor) -> None:
+    for name, t in operands.items():
+        heads, T = (a.Hk, a.Tk) if name in ("dk", "dv") else (a.H, a.Tq)
+        setattr(a, "s_" + name, _operand(t, name, (a.B, T, heads, a.D), q, name != "dout"))
+        setattr(a, name, t.data_ptr())
+
+
+def _check_lse(lse: torch.Tensor, a: _Args, q: torch.Tensor) -> None:
+    if (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device
+            or tuple(lse.shape) != (a.B, a.H, a.Tq)):
+        raise DeviceError(f"attention: lse must be contiguous float32 [{a.B}, {a.H}, {a.Tq}] on {q.device}")
+
+
+def _launch(a: _Args, q: torch.Tensor, backward: bool) -> None:
+    with library.on_device(q.device):
+        library.check(_fn("nf_attention")(byref(a), _TYPES[q.dtype], int(backward),
+                                          library.stream_ptr(q.device)),
+                      "attention_bwd" if backward else "attention_fwd")
+
+
+def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor | None = None,
+                  lse: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None,
+                  q_lengths: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None,
+                  dropout: float = 0.0, seed: int = 0, step: "int | torch.Tensor" = 0,
+                  first_batch: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """``out = drop(softmax(scale q k^T)) v`` per head and the log-sum-exp of every score row;
+    returns ``(out, lse)``.
+
+    ``q`` ``[B, Tq, H, D]``, ``k`` / ``v`` ``[B, Tk, Hk, D]``: bfloat16 or float16 with contiguous
+    columns, the other distances free (multiples of 8 elements, 16-byte aligned: views of a packed
+    projection or of a longer cache do).  Query head h reads key head ``h // (H // Hk)``.  ``D`` is a
+    multiple of 8 up to 128; ``scale`` is ``D ** -0.5`` by default.
+
+    ``q_lengths`` / ``k_lengths`` (int32 ``[B]`` on the device, taken to ``[0, T]``): sequence b has
+    that many queries and keys, right-padded; what lies behind them is not used and may hold
+    anything.  With ``causal`` the last query sees every key: key j is seen by query i where
+    ``j <= i + keys - queries`` (equal numbers: the usual triangle; one query: all of the cache).
+    Queries behind the length and queries that see no key give 0 and a log-sum-exp of -inf.  A
+    non-finite value that some query sees may spread to other queries of its sequence.
+
+    ``dropout`` (taken to a multiple of 1 / 256): each probability is dropped with it, what stays is
+    scaled by the inverse of the share that stays.  The mask is a function of ``seed``, ``step`` (a
+    number, or one int64 on the device that the kernel reads when it runs) and of the sequence, head,
+    query and key: probability (i, j) of head h of sequence b takes byte ``j & 3`` of word ``i & 3`` of
+    the Philox4x32-7 block with counter ``(j >> 2, i >> 2, (first_batch + b) H + h, step)``."""
+    a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
+    _add(a, q, out=out)
+    _check_lse(lse, a, q)
+    if q.numel() == 0:
+        return out, lse
+    if a.Tk == 0:
+        out.zero_()
+        lse.fill_(float("-inf"))
+        return out, lse
+    if q.device.type != "cuda":
+        prob, kept, sums = _probabilities(a, q, k, q_lengths, k_lengths, step)
+        lse.copy_(sums)
+        y = (prob * kept) @ _shared(a, v, k_lengths)
+        out.copy_(y.transpose(1, 2))
+        return out, lse
+    a.lse = lse.data_ptr()
+    _launch(a, q, False)
+    return out, lse
+
+
+def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                  lse: torch.Tensor, dout: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor,
+                  dv: torch.Tensor, *, causal: bool = True, scale: float | None = None,
+                  q_lengths: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None,
+                  dropout: float = 0.0, seed: int = 0, step: "int | torch.Tensor" = 0,
+                  first_batch: int = 0) -> None:
+    """Gradients of ``attention_fwd`` (called with the same arguments) from ``dout``: ``dq``, ``dk``,
+    ``dv`` are written everywhere, with 0 behind the lengths.  The probabilities are computed again
+    from ``lse`` and the mask from its counter; a key head's gradient is summed over the query heads
+    that share it in a fixed order, without atomics.  ``dq``, ``dk``, ``dv`` must not overlap what is
+    read."""
+    a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
+    _add(a, q, out=out, dout=dout, dq=dq, dk=dk, dv=dv)
+    _check_lse(lse, a, q)
+    if q.numel() == 0 or a.Tk == 0:
+        for t in (dq, dk, dv):
+            t.zero_()
+        return
+    if q.device.type != "cuda":
+        prob, kept, _ = _probabilities(a, q, k, q_lengths, k_lengths, step)
+        rows = _valid(a, q_lengths, a.Tq).view(a.B, 1, a.Tq, 1)
+        qf = _masked(q, rows)
+        do, o = _masked(dout, rows), _masked(out, rows)
+        kf, vf = _shared(a, k, k_lengths), _shared(a, v, k_lengths)
+        gv = (prob * kept).transpose(-1, -2) @ do
+        ds = prob * (do @ vf.transpose(-1, -2) * kept - (do * o).sum(-1, keepdim=True)) * a.scale
+        dq.copy_((ds @ kf).transpose(1, 2))
+        for t, g in ((dk, ds.transpose(-1, -2) @ qf), (dv, gv)):
+            t.copy_(g.view(a.B, a.Hk, a.H // a.Hk, a.Tk, a.D).sum(2).transpose(1, 2))
+        return
+    delta = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
+    a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
+    _launch(a, q, True)
+
+
+def _valid(a: _Args, lengths: torch.Tensor | None, T: int) -> torch.Tensor:
+    n = torch.full((a.B,), T) if lengths is None else lengths.clamp(0, T).long()
+    return torch.arange(T) < n[:, None]
+
+
+def _masked(t: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    """``[B, heads, T, D]`` in fp32 (double stays), rows that are not there as zeros."""
+    x = t if t.dtype == torch.float64 else t.float()
+    return torch.where(rows, x.transpose(1, 2), torch.zeros((), dtype=x.dtype))
+
+
+def _shared(a: _Args, t: torch.Tensor, lengths: torch.Tensor | None) -> torch.Tensor:
+    x = _masked(t, _valid(a, lengths, a.Tk).view(a.B, 1, a.Tk, 1))
+    return x.repeat_interleave(a.H // a.Hk, 1)
+
+
+def _probabilities(a: _Args, q, k, q_lengths, k_lengths, step):
+    """CPU: (probabilities, what each is multiplied by, log-sum-exp), ``[B, H, Tq, Tk]``."""
+    rows, keys = _valid(a, q_lengths, a.Tq), _valid(a, k_lengths, a.Tk)
+    seen = rows[:, :, None] & keys[:, None, :]
+    if a.causal:
+        off = (keys.sum(1) - rows.sum(1))[:, None, None]
+        seen = seen & (torch.arange(a.Tk) <= torch.arange(a.Tq)[:, None] + off)
+    qf = _masked(q, rows.view(a.B, 1, a.Tq, 1))
+    scores = (qf @ _shared(a, k, k_lengths).transpose(-1, -2)) * a.scale
+    scores = scores.masked_fill(~seen[:, None], float("-inf"))
+    sums = torch.logsumexp(scores, -1)
+    prob = torch.exp(scores - sums.masked_fill(sums == float("-inf"), 0.0)[..., None])
+    return prob, kept_pairs(a, step).to(prob.dtype) * a.up if a.limit else 1.0, sums
+
+
+def kept_pairs(a: _Args, step: "int | torch.Tensor") -> torch.Tensor:
+    """Whether each probability ``[B, H, Tq, Tk]`` is kept (CPU)."""
+    nq, nk = (a.Tq + 3) // 4, (a.Tk + 3) // 4
+    heads = (a.first_head + torch.arange(a.B * a.H).view(-1, 1, 1)) & 0xFFFFFFFF
+    w = philox_words(a.seed, step, torch.arange(nk), torch.arange(nq).view(-1, 1), heads)
+    b = w.transpose(2, 3).unsqueeze(-1) >> torch.tensor([0, 8, 16, 24]) & 0xFF
+    return (b >= a.limit).reshape(a.B, a.H, nq * 4, nk * 4)[:, :, : a.Tq, : a.Tk]

@@ -8,6 +8,7 @@ silently - a missing or unloadable library raises ``DeviceError``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_float, c_int, c_long, c_ulonglong, c_void_p
@@ -88,6 +89,17 @@ def declare(name: str, argtypes: list, restype=c_int):
 def stream_ptr(device: torch.device | None = None) -> c_void_p:
     """The current HIP stream of ``device`` as a ``hipStream_t``."""
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which launches go to ``device`` (a kernel is launched on the current device,
+    whatever stream it is given); free when that is the current one already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
 
 
 # NANOFED_DEBUG_SYNC=1: wait for the device after every native launch, so that an

@@ -60,7 +60,9 @@ __device__ __forceinline__ halfx4 tr4(const half* p) {
     return __builtin_bit_cast(halfx4, v);
 }
 
-constexpr int kStage = 64;  // keys (or queries) per LDS stage
+constexpr int kStage = 64;  // keys per LDS stage of the forward kernel
+// keys (or queries) per LDS stage of the backward kernels
+template <int DP> constexpr int kBwdStage = DP == 64 ? 64 : 32;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Strides { long b, t, h; };  // elements between sequences, rows, heads
@@ -82,48 +84,97 @@ struct AttnArgs {
     unsigned limit, step;
 };
 
-// -- LDS tiles: 64 rows of DP columns --------------------------------------------------------
-template <class E, int DP>
+// -- tiles ------------------------------------------------------------------------------------
+// R rows of DP columns in LDS.  They come through registers by buffer loads: the descriptor starts
+// at the tile's first row and ends with the last row there is, so rows behind it (and, by an offset
+// beyond any tile, columns behind D) read as 0 without a comparison, and a lane keeps one 32-bit
+// offset per piece for the whole loop.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <class E, int DP, int R>
 struct Tile {
     typedef typename Vec<E>::x8 x8;
     typedef typename Vec<E>::x4 x4;
-    static constexpr int kBytes = kStage * DP * 2;
-    static constexpr int kPieces = DP / 8;                 // 16-byte pieces of a row
-    static constexpr int kPer = kStage * kPieces / 256;    // ... per thread (256 threads)
-    struct Regs { uint4 v[kPer]; };
+    static constexpr int kRow = DP * 2, kBytes = R * kRow;
+    static constexpr int kPieces = DP / 8;             // 16-byte pieces of a row
+    static constexpr int kPer = R * kPieces / 256;     // ... per thread (256 threads)
+    struct Regs { u32x4 v[kPer]; };
+    struct From {                                      // a matrix that is walked tile by tile
+        const E* base;
+        long ld;
+        int rows, D;
+        unsigned off[kPer];
+    };
 
-    // rows [r0, r0 + 64) of a matrix with `rows` rows and D columns; the rest reads as 0
-    static __device__ __forceinline__ Regs load(const E* base, long ld, int r0, int rows, int D, int tid) {
+    static __device__ __forceinline__ From from(const void* p, long first, long ld, int rows, int D, int tid) {
+        From f = {static_cast<const E*>(p) + first, ld, rows, D, {}};
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int idx = tid + 256 * i, c = (idx % kPieces) * 8;
+            f.off[i] = c < D ? static_cast<unsigned>((idx / kPieces) * ld + c) * 2u : 0x80000000u;
+        }
+        return f;
+    }
+    static __device__ __forceinline__ Regs load(const From& f, int tile) {
+        const int left = f.rows - tile * R;
+        const long bytes = left > 0 ? ((min(left, R) - 1) * f.ld + f.D) * 2 : 0;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<E*>(f.base + tile * R * f.ld), 0, static_cast<int>(bytes), 0x00020000);
         Regs t;
 #pragma unroll
-        for (int p = 0; p < kPer; ++p) {
-            const int idx = tid + 256 * p, r = r0 + idx / kPieces, c = (idx % kPieces) * 8;
-            t.v[p] = make_uint4(0, 0, 0, 0);
-            if (r < rows && c < D) t.v[p] = *reinterpret_cast<const uint4*>(base + r * ld + c);
-        }
+        for (int i = 0; i < kPer; ++i)
+            t.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(f.off[i]), 0, 0);
         return t;
     }
     static __device__ __forceinline__ void store(char* lds, const Regs& t, int tid) {
 #pragma unroll
-        for (int p = 0; p < kPer; ++p) {
-            const int idx = tid + 256 * p;
-            *reinterpret_cast<uint4*>(lds + nfix::attn_off(DP, idx / kPieces, idx % kPieces)) = t.v[p];
+        for (int i = 0; i < kPer; ++i) {
+            const int idx = tid + 256 * i;
+            *reinterpret_cast<u32x4*>(lds + nfix::attn_off(DP, idx / kPieces, idx % kPieces)) = t.v[i];
         }
     }
-    // operand fragment: row `row`, columns 16 ks + 8 (lane >> 5) .. + 7
-    static __device__ __forceinline__ x8 row(const char* lds, int row, int ks, int hh) {
-        return *reinterpret_cast<const x8*>(lds + nfix::attn_off(DP, row, 2 * ks + hh));
+
+    // Operand fragments.  The permutation of the pieces has a period of 16 rows, so a lane's
+    // offsets within 16 (or 32) rows are computed once and the rest is a constant.
+    struct Lane {
+        int row[DP / 16];     // row (lane & 31), columns 16 ks + 8 (lane >> 5) .. + 7
+        int tr[DP / 32][2];   // transposing reads of columns 32 i + (lane & 31)
+    };
+    static __device__ __forceinline__ Lane lane_offsets(int lane) {
+        Lane o;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) o.row[ks] = nfix::attn_off(DP, lane & 31, 2 * ks + (lane >> 5));
+        const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2), x = 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j) {
+            o.tr[j][0] = nfix::attn_off(DP, r, (32 * j + x) >> 3) + (x & 7) * 2;
+            o.tr[j][1] = nfix::attn_off(DP, r + 8, (32 * j + x) >> 3) + (x & 7) * 2;
+        }
+        return o;
     }
-    // 8 values tile[k0 + (j & 3) + 4 h + 8 (j >> 2)][x0 + (lane & 31)], h = lane >> 5: rows in the
-    // order in which an accumulator hands them to the next MFMA
-    static __device__ __forceinline__ x8 tr(const char* lds, int k0, int x0, int lane) {
-        const int i = lane & 15;
-        const int r = k0 + 4 * (lane >> 5) + (i >> 2), x = x0 + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
-        const x4 lo = tr4(reinterpret_cast<const E*>(lds + nfix::attn_off(DP, r, x >> 3) + (x & 7) * 2));
-        const x4 hi = tr4(reinterpret_cast<const E*>(lds + nfix::attn_off(DP, r + 8, x >> 3) + (x & 7) * 2));
+    // rows row0 + (lane & 31); row0 a multiple of 32
+    static __device__ __forceinline__ x8 row(const char* lds, const Lane& o, int row0, int ks) {
+        return *reinterpret_cast<const x8*>(lds + row0 * kRow + o.row[ks]);
+    }
+    // 8 values tile[k0 + (j & 3) + 4 h + 8 (j >> 2)][32 i + (lane & 31)], h = lane >> 5, k0 a multiple
+    // of 16: rows in the order in which an accumulator hands them to the next MFMA
+    static __device__ __forceinline__ x8 tr(const char* lds, const Lane& o, int k0, int i) {
+        const x4 lo = tr4(reinterpret_cast<const E*>(lds + k0 * kRow + o.tr[i][0]));
+        const x4 hi = tr4(reinterpret_cast<const E*>(lds + k0 * kRow + o.tr[i][1]));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
+
+// rows [.., D) of a lane's own row as operand fragments, 0 where there is no row or column
+template <class E, int DP>
+__device__ __forceinline__ void own_row(const E* p, bool there, int D, int hh, typename Vec<E>::x8 (&f)[DP / 16]) {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        f[ks] = {};
+        const int c = ks * 16 + 8 * hh;
+        if (there && c < D) f[ks] = *reinterpret_cast<const typename Vec<E>::x8*>(p + c);
+    }
+}
 
 template <class E>
 __device__ __forceinline__ typename Vec<E>::x8 pack8(const f32x16& v, int first) {
@@ -186,6 +237,23 @@ __device__ __forceinline__ bool kept(const unsigned (&w)[4], int r, unsigned lim
     return ((w[r >> 2] >> (8 * (r & 3))) & 0xFFu) >= limit;
 }
 
+// Tiles that every query of the wave sees whole are most of them; without this the comparisons
+// of the others would be turned into selects that all tiles pay for.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
+// row of accumulator register r without the lane's part (4 (lane >> 5))
+__device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// of a lane and its other half (lane ^ 32)
+__device__ __forceinline__ float max_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // -- what a workgroup knows about its sequence -------------------------------------------------
 struct Seq { int m, n, off; };  // queries, keys, and: query i sees keys j <= i + off
 
@@ -209,240 +277,265 @@ __device__ __forceinline__ unsigned step_of(const AttnArgs& a) {
 // buffered in LDS.  grid = (sequence and head, tile): the tiles of a head land on one XCD, the
 // long ones are dispatched first.
 template <class E, int DP, bool kDrop>
-__global__ void __launch_bounds__(256) attn_fwd_kernel(AttnArgs a) {
-    typedef Tile<E, DP> T;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 3 : 2)))
+attn_fwd_kernel(AttnArgs a) {
+    typedef Tile<E, DP, kStage> T;
     typedef typename T::x8 x8;
+    constexpr int NB = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const int tile0 = (gridDim.y - 1 - blockIdx.y) * 128;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
-    const E* qb = static_cast<const E*>(a.q) + b * a.sq.b + h * a.sq.h;
-    const E* kb = static_cast<const E*>(a.k) + b * a.sk.b + hk * a.sk.h;
-    const E* vb = static_cast<const E*>(a.v) + b * a.sv.b + hk * a.sv.h;
     const int q0 = tile0 + wave * 32, qi = q0 + n;
     const int stages = tile0 < sq.m ? (keys_seen(sq, min(tile0 + 127, sq.m - 1)) + kStage - 1) / kStage : 0;
+    const typename T::From kfrom = T::from(a.k, b * a.sk.b + hk * a.sk.h, a.sk.t, sq.n, a.D, tid);
+    const typename T::From vfrom = T::from(a.v, b * a.sv.b + hk * a.sv.h, a.sv.t, sq.n, a.D, tid);
+    const typename T::Lane at = T::lane_offsets(lane);
     x8 qf[DP / 16];
+    own_row<E, DP>(static_cast<const E*>(a.q) + b * a.sq.b + h * a.sq.h + qi * a.sq.t, qi < sq.m, a.D, hh, qf);
+    f32x16 o[NB];
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-        qf[ks] = {};
-        const int c = ks * 16 + 8 * hh;
-        if (qi < sq.m && c < a.D) qf[ks] = *reinterpret_cast<const x8*>(qb + qi * a.sq.t + c);
-    }
-    f32x16 o[DP / 32];
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{0};
-    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < NB; ++i) o[i] = f32x16{0};
+    float m = -INFINITY, l = 0.f, msc = 0.f;  // running maximum, sum, and maximum in the exponent
     const float sc2 = a.scale * kLog2e;
-    // keys that the wave's first and last query see, and this lane's
-    const int seen_lo = keys_seen(sq, q0), seen = keys_seen(sq, qi);
-    const int seen_hi = q0 < sq.m ? keys_seen(sq, q0 + 31) : 0;
+    // keys that the wave's first and last query see, and this lane's (less its rows' offset)
+    const int seen_lo = __builtin_amdgcn_readfirstlane(keys_seen(sq, q0)), seen = keys_seen(sq, qi) - 4 * hh;
+    const int seen_hi = __builtin_amdgcn_readfirstlane(q0 < sq.m ? keys_seen(sq, q0 + 31) : 0);
     const unsigned step = kDrop ? step_of(a) : 0u, head = static_cast<unsigned>(a.first_head + bh);
 
     typename T::Regs kr, vr;
-    if (stages > 0) {
-        kr = T::load(kb, a.sk.t, 0, sq.n, a.D, tid);
-        vr = T::load(vb, a.sv.t, 0, sq.n, a.D, tid);
-        T::store(smem, kr, tid);
-        T::store(smem + 2 * T::kBytes, vr, tid);
-    }
-    __syncthreads();
-    for (int st = 0; st < stages; ++st) {
-        const char* Ks = smem + (st & 1) * T::kBytes;
-        const char* Vs = smem + (2 + (st & 1)) * T::kBytes;
-        if (st + 1 < stages) {
-            kr = T::load(kb, a.sk.t, (st + 1) * kStage, sq.n, a.D, tid);
-            vr = T::load(vb, a.sv.t, (st + 1) * kStage, sq.n, a.D, tid);
+    auto tile = [&](const char* Ks, const char* Vs, int key0) {
+        f32x16 s[2] = {{0}, {0}};
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) s[sub] = mma(T::row(Ks, at, sub * 32, ks), qf[ks], s[sub]);
+        if (key0 + kStage > seen_lo) {  // wave-uniform: some pair of the tile is not visible
+            keep_branch();
+            const int lim = seen - key0;
+#pragma unroll
+            for (int r = 0; r < 32; ++r)
+                if (reg_row(r & 15) + 32 * (r >> 4) >= lim) s[r >> 4][r & 15] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+        mx = max_halves(mx);
+        if (__any(mx > m)) {  // the running maximum rarely moves after the first tiles
+            const float mn = fmaxf(m, mx);
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            const float alpha = exp2_fast((m - ref) * sc2);
+            m = mn;
+            msc = ref * sc2;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
         }
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
-            const int key0 = st * kStage + sub * 32;
-            if (key0 >= seen_hi) continue;  // wave-uniform: nothing visible in this tile
-            f32x16 s = {0};
+            float r0 = 0.f, r1 = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) s = mma(T::row(Ks, sub * 32 + n, ks, hh), qf[ks], s);
-            if (key0 + 32 > seen_lo) {      // wave-uniform: some pair of the tile is not visible
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (key0 + acc_row(r, lane) >= seen) s[r] = -INFINITY;
+            for (int r = 0; r < 16; r += 2) {
+                s[sub][r] = exp2_fast(fmaf(s[sub][r], sc2, -msc));
+                s[sub][r + 1] = exp2_fast(fmaf(s[sub][r + 1], sc2, -msc));
+                r0 += s[sub][r];
+                r1 += s[sub][r + 1];
             }
-            float mx = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            if (__any(mx > m)) {  // the running maximum rarely moves after the first tiles
-                const float mn = fmaxf(m, mx);
-                const float ref = mn == -INFINITY ? 0.f : mn;
-                const float alpha = exp2_fast((m - ref) * sc2);
-                m = mn;
-                l *= alpha;
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
-            }
-            const float msc = m == -INFINITY ? 0.f : m * sc2;
-            float rs = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = exp2_fast(fmaf(s[r], sc2, -msc));
-                rs += s[r];
-            }
-            l += rs;
+            l += r0 + r1;
             if (kDrop) {  // the sum is of all probabilities, what is dropped leaves the product
                 unsigned w[4];
-                mask_bytes<true>(w, a.seed, head, step, key0, q0, lane);
+                mask_bytes<true>(w, a.seed, head, step, key0 + 32 * sub, q0, lane);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!kept(w, r, a.limit)) s[r] = 0.f;
+                    if (!kept(w, r, a.limit)) s[sub][r] = 0.f;
             }
-            const x8 p0 = pack8<E>(s, 0), p1 = pack8<E>(s, 8);
+            const x8 p0 = pack8<E>(s[sub], 0), p1 = pack8<E>(s[sub], 8);
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                o[i] = mma(T::tr(Vs, sub * 32, 32 * i, lane), p0, o[i]);
-                o[i] = mma(T::tr(Vs, sub * 32 + 16, 32 * i, lane), p1, o[i]);
+            for (int i = 0; i < NB; ++i) {
+                o[i] = mma(T::tr(Vs, at, sub * 32, i), p0, o[i]);
+                o[i] = mma(T::tr(Vs, at, sub * 32 + 16, i), p1, o[i]);
             }
         }
+    };
+    auto stage = [&](int st, char* here, char* there) {
         if (st + 1 < stages) {
-            T::store(smem + ((st + 1) & 1) * T::kBytes, kr, tid);
-            T::store(smem + (2 + ((st + 1) & 1)) * T::kBytes, vr, tid);
+            kr = T::load(kfrom, st + 1);
+            vr = T::load(vfrom, st + 1);
+        }
+        if (st * kStage < seen_hi) tile(here, here + T::kBytes, st * kStage);  // wave-uniform
+        if (st + 1 < stages) {
+            T::store(there, kr, tid);
+            T::store(there + T::kBytes, vr, tid);
         }
         __syncthreads();
+    };
+    if (stages > 0) {
+        kr = T::load(kfrom, 0);
+        vr = T::load(vfrom, 0);
+        T::store(smem, kr, tid);
+        T::store(smem + T::kBytes, vr, tid);
+    }
+    __syncthreads();
+    for (int st = 0; st < stages; st += 2) {
+        stage(st, smem, smem + 2 * T::kBytes);
+        if (st + 1 < stages) stage(st + 1, smem + 2 * T::kBytes, smem);
     }
     if (qi >= a.Tq) return;
-    l += __shfl_xor(l, 32, 64);
-    const bool some = qi < sq.m && l > 0.f;
-    const float inv = some || l != l ? (kDrop ? a.up : 1.f) / l : 0.f;
+    l = sum_halves(l);
+    const bool some = qi < sq.m && (l > 0.f || l != l);
+    const float inv = some ? (kDrop ? a.up : 1.f) / l : 0.f;
     E* orow = static_cast<E*>(a.out) + b * a.so.b + qi * a.so.t + h * a.so.h;
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             typename T::x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(qi < sq.m ? o[i][4 * g + e] * inv : 0.f);
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(some ? o[i][4 * g + e] * inv : 0.f);
             const int c = 32 * i + 8 * g + 4 * hh;
             if (c < a.D) *reinterpret_cast<typename T::x4*>(orow + c) = v;
         }
     if (hh == 0)
-        a.lse[static_cast<long>(bh) * a.Tq + qi] =
-            qi < sq.m && (some || l != l) ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+        a.lse[static_cast<long>(bh) * a.Tq + qi] = some ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------
-// Backward, queries: one workgroup = 128 queries; streams K / V.  Also leaves D = rowsum(dO * O)
-// for the dK / dV kernel that follows.
+// Backward, queries: one workgroup = 128 queries; streams K / V.
+//
+// D = rowsum(dO * O) takes O as it was stored: rounded, and summed from rounded probabilities.
+// Its error is the same for all keys of a row, so it would come back as error * (P K) in dQ and
+// make dQ and dK half as far off again as the two roundings that they cannot do without.  But
+// sum_j dS_ij = 0 in exact arithmetic, so the row's sum r = sum_j dS_ij, which costs one addition
+// per pair in fp32, is that error: dQ is corrected by -r (P K), at the cost of a fourth product,
+// and the dK / dV kernel that follows gets D + r.
 template <class E, int DP, bool kDrop>
-__global__ void __launch_bounds__(256) attn_dq_kernel(AttnArgs a) {
-    typedef Tile<E, DP> T;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
+attn_dq_kernel(AttnArgs a) {
+    constexpr int R = kBwdStage<DP>, NB = DP / 32;
+    typedef Tile<E, DP, R> T;
     typedef typename T::x8 x8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const int tile0 = (gridDim.y - 1 - blockIdx.y) * 128;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
-    const E* qb = static_cast<const E*>(a.q) + b * a.sq.b + h * a.sq.h;
-    const E* kb = static_cast<const E*>(a.k) + b * a.sk.b + hk * a.sk.h;
-    const E* vb = static_cast<const E*>(a.v) + b * a.sv.b + hk * a.sv.h;
-    const E* ob = static_cast<const E*>(a.out) + b * a.so.b + h * a.so.h;
-    const E* dob = static_cast<const E*>(a.dout) + b * a.sdo.b + h * a.sdo.h;
     const int q0 = tile0 + wave * 32, qi = q0 + n;
-    const int stages = tile0 < sq.m ? (keys_seen(sq, min(tile0 + 127, sq.m - 1)) + kStage - 1) / kStage : 0;
+    const bool in = qi < sq.m;
+    const int stages = tile0 < sq.m ? (keys_seen(sq, min(tile0 + 127, sq.m - 1)) + R - 1) / R : 0;
+    const typename T::From kfrom = T::from(a.k, b * a.sk.b + hk * a.sk.h, a.sk.t, sq.n, a.D, tid);
+    const typename T::From vfrom = T::from(a.v, b * a.sv.b + hk * a.sv.h, a.sv.t, sq.n, a.D, tid);
+    const typename T::Lane at = T::lane_offsets(lane);
     x8 qf[DP / 16], df[DP / 16];
+    own_row<E, DP>(static_cast<const E*>(a.q) + b * a.sq.b + h * a.sq.h + qi * a.sq.t, in, a.D, hh, qf);
+    own_row<E, DP>(static_cast<const E*>(a.dout) + b * a.sdo.b + h * a.sdo.h + qi * a.sdo.t, in, a.D, hh, df);
     float delta = 0.f;
+    {
+        x8 of[DP / 16];
+        own_row<E, DP>(static_cast<const E*>(a.out) + b * a.so.b + h * a.so.h + qi * a.so.t, in, a.D, hh, of);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-        qf[ks] = {};
-        df[ks] = {};
-        const int c = ks * 16 + 8 * hh;
-        if (qi < sq.m && c < a.D) {
-            qf[ks] = *reinterpret_cast<const x8*>(qb + qi * a.sq.t + c);
-            df[ks] = *reinterpret_cast<const x8*>(dob + qi * a.sdo.t + c);
-            const x8 of = *reinterpret_cast<const x8*>(ob + qi * a.so.t + c);
+        for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                delta = fmaf(static_cast<float>(df[ks][j]), static_cast<float>(of[j]), delta);
-        }
+                delta = fmaf(static_cast<float>(df[ks][j]), static_cast<float>(of[ks][j]), delta);
     }
-    delta += __shfl_xor(delta, 32, 64);
-    const long at = static_cast<long>(bh) * a.Tq + qi;
+    delta = sum_halves(delta);
+    const long row = static_cast<long>(bh) * a.Tq + qi;
     // a row that sees no key has lse -inf: +inf makes its probabilities 0
-    float lse2 = INFINITY;
-    if (qi < sq.m) {
-        const float v = a.lse[at];
-        lse2 = v == -INFINITY ? INFINITY : v * kLog2e;
-    }
-    if (qi < a.Tq && hh == 0) a.delta[at] = delta;
-    f32x16 dq[DP / 32];
+    float lse2 = in ? a.lse[row] : -INFINITY;
+    lse2 = lse2 == -INFINITY ? INFINITY : lse2 * kLog2e;
+    f32x16 dq[NB], pk[NB];
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) dq[i] = f32x16{0};
+    for (int i = 0; i < NB; ++i) { dq[i] = f32x16{0}; pk[i] = f32x16{0}; }
+    float off = 0.f;  // sum of dS
     const float sc2 = a.scale * kLog2e;
-    const int seen_lo = keys_seen(sq, q0), seen = keys_seen(sq, qi);
-    const int seen_hi = q0 < sq.m ? keys_seen(sq, q0 + 31) : 0;
+    const int seen_lo = __builtin_amdgcn_readfirstlane(keys_seen(sq, q0)), seen = keys_seen(sq, qi) - 4 * hh;
+    const int seen_hi = __builtin_amdgcn_readfirstlane(q0 < sq.m ? keys_seen(sq, q0 + 31) : 0);
     const unsigned step = kDrop ? step_of(a) : 0u, head = static_cast<unsigned>(a.first_head + bh);
 
     typename T::Regs kr, vr;
-    if (stages > 0) {
-        kr = T::load(kb, a.sk.t, 0, sq.n, a.D, tid);
-        vr = T::load(vb, a.sv.t, 0, sq.n, a.D, tid);
-        T::store(smem, kr, tid);
-        T::store(smem + 2 * T::kBytes, vr, tid);
-    }
-    __syncthreads();
-    for (int st = 0; st < stages; ++st) {
-        const char* Ks = smem + (st & 1) * T::kBytes;
-        const char* Vs = smem + (2 + (st & 1)) * T::kBytes;
-        if (st + 1 < stages) {
-            kr = T::load(kb, a.sk.t, (st + 1) * kStage, sq.n, a.D, tid);
-            vr = T::load(vb, a.sv.t, (st + 1) * kStage, sq.n, a.D, tid);
+    auto tile = [&](const char* Ks, const char* Vs, int key0) {
+        f32x16 s = {0}, dp = {0};
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+            s = mma(T::row(Ks, at, 0, ks), qf[ks], s);
+            dp = mma(T::row(Vs, at, 0, ks), df[ks], dp);
         }
+        unsigned w[4];
+        if (kDrop) mask_bytes<true>(w, a.seed, head, step, key0, q0, lane);
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            const int key0 = st * kStage + sub * 32;
-            if (key0 >= seen_hi) continue;
-            f32x16 s = {0}, dp = {0};
+        for (int r = 0; r < 16; ++r) {
+            s[r] = exp2_fast(fmaf(s[r], sc2, -lse2));
+            if (kDrop) dp[r] = fmaf(dp[r], kept(w, r, a.limit) ? a.up : 0.f, -delta);
+            else dp[r] -= delta;
+        }
+        if (key0 + 32 > seen_lo) {  // wave-uniform: some pair of the tile is not visible
+            keep_branch();
+            const int lim = seen - key0;
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                s = mma(T::row(Ks, sub * 32 + n, ks, hh), qf[ks], s);
-                dp = mma(T::row(Vs, sub * 32 + n, ks, hh), df[ks], dp);
-            }
-            unsigned w[4];
-            if (kDrop) mask_bytes<true>(w, a.seed, head, step, key0, q0, lane);
-            const bool edge = key0 + 32 > seen_lo;
+            for (int r = 0; r < 16; ++r)
+                if (reg_row(r) >= lim) { s[r] = 0.f; dp[r] = 0.f; }
+        }
+        float t = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = exp2_fast(fmaf(s[r], sc2, -lse2));
-                float d = dp[r];
-                if (kDrop) d = kept(w, r, a.limit) ? d * a.up : 0.f;
-                s[r] = p * (d - delta);
-            }
-            if (edge) {
+        for (int r = 0; r < 16; ++r) {
+            dp[r] *= s[r];
+            t += dp[r];
+        }
+        off += t;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (key0 + acc_row(r, lane) >= seen) s[r] = 0.f;
-            }
-            const x8 s0 = pack8<E>(s, 0), s1 = pack8<E>(s, 8);
+        for (int g = 0; g < 2; ++g) {
+            const x8 ds = pack8<E>(dp, 8 * g), p = pack8<E>(s, 8 * g);
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                dq[i] = mma(T::tr(Ks, sub * 32, 32 * i, lane), s0, dq[i]);
-                dq[i] = mma(T::tr(Ks, sub * 32 + 16, 32 * i, lane), s1, dq[i]);
+            for (int i = 0; i < NB; ++i) {
+                const x8 k = T::tr(Ks, at, 16 * g, i);
+                dq[i] = mma(k, ds, dq[i]);
+                pk[i] = mma(k, p, pk[i]);
             }
         }
+    };
+    auto stage = [&](int st, char* here, char* there) {
         if (st + 1 < stages) {
-            T::store(smem + ((st + 1) & 1) * T::kBytes, kr, tid);
-            T::store(smem + (2 + ((st + 1) & 1)) * T::kBytes, vr, tid);
+            kr = T::load(kfrom, st + 1);
+            vr = T::load(vfrom, st + 1);
+        }
+#pragma unroll
+        for (int sub = 0; sub < R / 32; ++sub)
+            if (st * R + sub * 32 < seen_hi)  // wave-uniform
+                tile(here + sub * 32 * T::kRow, here + T::kBytes + sub * 32 * T::kRow, st * R + sub * 32);
+        if (st + 1 < stages) {
+            T::store(there, kr, tid);
+            T::store(there + T::kBytes, vr, tid);
         }
         __syncthreads();
+    };
+    if (stages > 0) {
+        kr = T::load(kfrom, 0);
+        vr = T::load(vfrom, 0);
+        T::store(smem, kr, tid);
+        T::store(smem + T::kBytes, vr, tid);
+    }
+    __syncthreads();
+    for (int st = 0; st < stages; st += 2) {
+        stage(st, smem, smem + 2 * T::kBytes);
+        if (st + 1 < stages) stage(st + 1, smem + 2 * T::kBytes, smem);
     }
     if (qi >= a.Tq) return;
+    off = sum_halves(off);
+    if (hh == 0) a.delta[row] = delta + off;
     E* drow = static_cast<E*>(a.dq) + b * a.sdq.b + qi * a.sdq.t + h * a.sdq.h;
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             typename T::x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(qi < sq.m ? dq[i][4 * g + e] * a.scale : 0.f);
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * g + e;
+                v[e] = static_cast<E>(in ? fmaf(-off, pk[i][r], dq[i][r]) * a.scale : 0.f);
+            }
             const int c = 32 * i + 8 * g + 4 * hh;
             if (c < a.D) *reinterpret_cast<typename T::x4*>(drow + c) = v;
         }
@@ -452,128 +545,140 @@ __global__ void __launch_bounds__(256) attn_dq_kernel(AttnArgs a) {
 // Backward, keys: one workgroup = 128 keys of one key head; streams Q / dO of every query head
 // that reads them.
 template <class E, int DP, bool kDrop>
-__global__ void __launch_bounds__(256) attn_dkdv_kernel(AttnArgs a) {
-    typedef Tile<E, DP> T;
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
+attn_dkdv_kernel(AttnArgs a) {
+    constexpr int R = kBwdStage<DP>, NB = DP / 32;
+    typedef Tile<E, DP, R> T;
     typedef typename T::x8 x8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int bh = blockIdx.x, b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
     const int tile0 = blockIdx.y * 128;  // key tile 0 is seen by every query: longest first
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
-    const E* kb = static_cast<const E*>(a.k) + b * a.sk.b + hk * a.sk.h;
-    const E* vb = static_cast<const E*>(a.v) + b * a.sv.b + hk * a.sv.h;
-    const int key0 = tile0 + wave * 32, kj = key0 + n;
+    const int key0 = __builtin_amdgcn_readfirstlane(tile0 + wave * 32), kj = key0 + n;
+    const typename T::Lane at = T::lane_offsets(lane);
     x8 kf[DP / 16], vf[DP / 16];
+    own_row<E, DP>(static_cast<const E*>(a.k) + b * a.sk.b + hk * a.sk.h + kj * a.sk.t, kj < sq.n, a.D, hh, kf);
+    own_row<E, DP>(static_cast<const E*>(a.v) + b * a.sv.b + hk * a.sv.h + kj * a.sv.t, kj < sq.n, a.D, hh, vf);
+    f32x16 dk[NB], dv[NB];
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-        kf[ks] = {};
-        vf[ks] = {};
-        const int c = ks * 16 + 8 * hh;
-        if (kj < sq.n && c < a.D) {
-            kf[ks] = *reinterpret_cast<const x8*>(kb + kj * a.sk.t + c);
-            vf[ks] = *reinterpret_cast<const x8*>(vb + kj * a.sv.t + c);
-        }
-    }
-    f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i) { dk[i] = f32x16{0}; dv[i] = f32x16{0}; }
+    for (int i = 0; i < NB; ++i) { dk[i] = f32x16{0}; dv[i] = f32x16{0}; }
     const float sc2 = a.scale * kLog2e;
     const unsigned step = kDrop ? step_of(a) : 0u;
     // query i sees key j from i >= j - off on
-    const int first = tile0 < sq.n ? max(0, a.causal ? tile0 - sq.off : 0) / kStage : 0;
-    const int stages = tile0 < sq.n ? (sq.m + kStage - 1) / kStage : 0;
-    const int per_head = max(0, stages - first), total = per_head * group;
+    const int first = tile0 < sq.n && a.causal ? max(0, tile0 - sq.off) / R : 0;
+    const int stages = tile0 < sq.n ? (sq.m + R - 1) / R : 0;
 
-    constexpr int kBuf = 2 * T::kBytes + 2 * kStage * 4;
+    constexpr int kBuf = 2 * T::kBytes + 2 * R * 4;
     typename T::Regs qr, dr;
     float ls = 0.f, de = 0.f;
-    auto fetch = [&](int it) {
-        const int h = hk * group + it / per_head, r0 = (first + it % per_head) * kStage;
-        qr = T::load(static_cast<const E*>(a.q) + b * a.sq.b + h * a.sq.h, a.sq.t, r0, sq.m, a.D, tid);
-        dr = T::load(static_cast<const E*>(a.dout) + b * a.sdo.b + h * a.sdo.h, a.sdo.t, r0, sq.m, a.D, tid);
-        if (tid < kStage) {
-            const long at = (static_cast<long>(b) * a.H + h) * a.Tq + r0 + tid;
-            const bool in = r0 + tid < sq.m;
-            ls = in ? a.lse[at] : -INFINITY;
-            ls = ls == -INFINITY ? INFINITY : ls * kLog2e;
-            de = in ? a.delta[at] : 0.f;
-        }
-    };
-    auto fill = [&](char* base) {
-        T::store(base, qr, tid);
-        T::store(base + T::kBytes, dr, tid);
-        if (tid < kStage) {
-            reinterpret_cast<float*>(base + 2 * T::kBytes)[tid] = ls;
-            reinterpret_cast<float*>(base + 2 * T::kBytes)[kStage + tid] = de;
-        }
-    };
-    if (total > 0) {
-        fetch(0);
-        fill(smem);
-    }
-    __syncthreads();
-    for (int it = 0; it < total; ++it) {
-        const char* Qs = smem + (it & 1) * kBuf;
-        const char* Ds = Qs + T::kBytes;
-        const float* lse2 = reinterpret_cast<const float*>(Qs + 2 * T::kBytes);
-        const float* del = lse2 + kStage;
-        const int st = first + it % per_head;
-        const unsigned head = static_cast<unsigned>(a.first_head + b * a.H + hk * group + it / per_head);
-        if (it + 1 < total) fetch(it + 1);
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            const int qs0 = st * kStage + sub * 32;
-            // wave-uniform: every query of the tile precedes every key, or there is none
-            if (qs0 + 31 + sq.off < key0 || qs0 >= sq.m) continue;
+    for (int g = 0; g < group; ++g) {
+        const int h = hk * group + g;
+        const typename T::From qfrom = T::from(a.q, b * a.sq.b + h * a.sq.h, a.sq.t, sq.m, a.D, tid);
+        const typename T::From dfrom = T::from(a.dout, b * a.sdo.b + h * a.sdo.h, a.sdo.t, sq.m, a.D, tid);
+        const long rows = (static_cast<long>(b) * a.H + h) * a.Tq;
+        const unsigned head = static_cast<unsigned>(a.first_head + b * a.H + h);
+        auto fetch = [&](int st) {
+            qr = T::load(qfrom, st);
+            dr = T::load(dfrom, st);
+            if (tid < R) {
+                const int i = st * R + tid;
+                ls = i < sq.m ? a.lse[rows + i] : -INFINITY;
+                de = i < sq.m ? a.delta[rows + i] : 0.f;
+            }
+        };
+        auto fill = [&](char* base) {
+            T::store(base, qr, tid);
+            T::store(base + T::kBytes, dr, tid);
+            if (tid < R) {
+                reinterpret_cast<float*>(base + 2 * T::kBytes)[tid] = ls == -INFINITY ? INFINITY : ls * kLog2e;
+                reinterpret_cast<float*>(base + 2 * T::kBytes)[R + tid] = de;
+            }
+        };
+        auto tile = [&](const char* Qs, const char* Ds, const float* lse2, const float* del, int qs0) {
             f32x16 s = {0}, dp = {0};
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) {
-                s = mma(T::row(Qs, sub * 32 + n, ks, hh), kf[ks], s);
-                dp = mma(T::row(Ds, sub * 32 + n, ks, hh), vf[ks], dp);
+                s = mma(T::row(Qs, at, 0, ks), kf[ks], s);
+                dp = mma(T::row(Ds, at, 0, ks), vf[ks], dp);
             }
             unsigned w[4];
             if (kDrop) mask_bytes<false>(w, a.seed, head, step, qs0, key0, lane);
-            const bool edge = qs0 + sq.off < key0 + 31;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 l4 = *reinterpret_cast<const float4*>(lse2 + sub * 32 + 8 * g + 4 * hh);
-                const float4 d4 = *reinterpret_cast<const float4*>(del + sub * 32 + 8 * g + 4 * hh);
-                const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse2 + 8 * q + 4 * hh);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * q + e] = exp2_fast(fmaf(s[4 * q + e], sc2, -l4[e]));
+            }
+            if (qs0 + sq.off < key0 + 31) {  // wave-uniform: some query of the tile precedes some key
+                keep_branch();
+                const int lim = kj - sq.off - qs0 - 4 * hh;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (reg_row(r) < lim) s[r] = 0.f;
+            }
+            f32x16 pd = s;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(del + 8 * q + 4 * hh);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * g + e;
-                    float p = exp2_fast(fmaf(s[r], sc2, -lv[e])), d = dp[r];
-                    if (edge && kj > qs0 + 8 * g + 4 * hh + e + sq.off) p = 0.f;
-                    const bool in = !kDrop || kept(w, r, a.limit);
-                    if (kDrop) d = in ? d * a.up : 0.f;
-                    s[r] = in ? p : 0.f;
-                    dp[r] = p * (d - dl[e]);
+                    const int r = 4 * q + e;
+                    if (kDrop) {
+                        const bool in = kept(w, r, a.limit);
+                        pd[r] = in ? s[r] : 0.f;
+                        dp[r] = s[r] * fmaf(dp[r], in ? a.up : 0.f, -d4[e]);
+                    } else {
+                        dp[r] = s[r] * (dp[r] - d4[e]);
+                    }
                 }
             }
-            const x8 p0 = pack8<E>(s, 0), p1 = pack8<E>(s, 8);
-            const x8 s0 = pack8<E>(dp, 0), s1 = pack8<E>(dp, 8);
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                dv[i] = mma(p0, T::tr(Ds, sub * 32, 32 * i, lane), dv[i]);
-                dv[i] = mma(p1, T::tr(Ds, sub * 32 + 16, 32 * i, lane), dv[i]);
-                dk[i] = mma(s0, T::tr(Qs, sub * 32, 32 * i, lane), dk[i]);
-                dk[i] = mma(s1, T::tr(Qs, sub * 32 + 16, 32 * i, lane), dk[i]);
+            for (int k = 0; k < 2; ++k) {
+                const x8 p = pack8<E>(pd, 8 * k), ds = pack8<E>(dp, 8 * k);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    dv[i] = mma(p, T::tr(Ds, at, 16 * k, i), dv[i]);
+                    dk[i] = mma(ds, T::tr(Qs, at, 16 * k, i), dk[i]);
+                }
             }
+        };
+        auto stage = [&](int st, char* here, char* there) {
+            if (st + 1 < stages) fetch(st + 1);
+            const float* lse2 = reinterpret_cast<const float*>(here + 2 * T::kBytes);
+#pragma unroll
+            for (int sub = 0; sub < R / 32; ++sub) {
+                const int qs0 = st * R + sub * 32;
+                // wave-uniform: every query of the tile precedes every key, or there is none
+                if (qs0 + 31 + sq.off >= key0 && qs0 < sq.m)
+                    tile(here + sub * 32 * T::kRow, here + T::kBytes + sub * 32 * T::kRow, lse2 + sub * 32,
+                         lse2 + R + sub * 32, qs0);
+            }
+            if (st + 1 < stages) fill(there);
+            __syncthreads();
+        };
+        if (first < stages) {
+            fetch(first);
+            fill(smem);
         }
-        if (it + 1 < total) fill(smem + ((it + 1) & 1) * kBuf);
         __syncthreads();
+        for (int st = first; st < stages; st += 2) {
+            stage(st, smem, smem + kBuf);
+            if (st + 1 < stages) stage(st + 1, smem + kBuf, smem);
+        }
     }
-    // register r of block i: key key0 + acc_row(r), column 32 i + n
+    // register r of block i: key key0 + acc_row(r), column 32 i + n.  (The factor of what is kept
+    // comes last: the probabilities are rounded without it, so that a probability of 1 stays exact.)
+    const float up = kDrop ? a.up : 1.f;
     E* dkb = static_cast<E*>(a.dk) + b * a.sdk.b + hk * a.sdk.h;
     E* dvb = static_cast<E*>(a.dv) + b * a.sdv.b + hk * a.sdv.h;
-    const float up = kDrop ? a.up : 1.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const int j = key0 + acc_row(r, lane);
         if (j >= a.Tk) continue;
         const bool in = j < sq.n;
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
+        for (int i = 0; i < NB; ++i) {
             const int c = 32 * i + n;
             if (c >= a.D) continue;
             dkb[j * a.sdk.t + c] = static_cast<E>(in ? dk[i][r] * a.scale : 0.f);
@@ -589,7 +694,7 @@ int set_lds(const void* fn, int bytes) {
 
 template <class E, int DP, bool kDrop>
 int launch_fwd(const AttnArgs& a, hipStream_t s) {
-    constexpr int lds = 4 * Tile<E, DP>::kBytes;
+    constexpr int lds = 4 * Tile<E, DP, kStage>::kBytes;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_fwd_kernel<E, DP, kDrop>), lds)) return st;
     hipLaunchKernelGGL((attn_fwd_kernel<E, DP, kDrop>), dim3(a.B * a.H, (a.Tq + 127) / 128), dim3(256), lds, s, a);
     return static_cast<int>(hipGetLastError());
@@ -597,7 +702,8 @@ int launch_fwd(const AttnArgs& a, hipStream_t s) {
 
 template <class E, int DP, bool kDrop>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {
-    constexpr int lds = 4 * Tile<E, DP>::kBytes, lds2 = lds + 4 * kStage * 4;
+    constexpr int rows = kBwdStage<DP>;
+    constexpr int lds = 4 * Tile<E, DP, rows>::kBytes, lds2 = lds + 4 * rows * 4;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop>), lds)) return st;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_dkdv_kernel<E, DP, kDrop>), lds2)) return st;
     hipLaunchKernelGGL((attn_dq_kernel<E, DP, kDrop>), dim3(a.B * a.H, (a.Tq + 127) / 128), dim3(256), lds, s, a);
@@ -613,7 +719,7 @@ int launch(const AttnArgs& a, int backward, hipStream_t s) {
 
 bool fits(const void* p, const Strides& st) {
     return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && st.b % 8 == 0 && st.t % 8 == 0 &&
-           st.h % 8 == 0;
+           st.h % 8 == 0 && st.t >= 0 && st.t < (1L << 24);
 }
 
 }  // namespace

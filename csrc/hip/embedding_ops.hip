@@ -48,91 +48,340 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(const long* tokens, 
     store_unit(out + r * C + c, n, f);
 }
 
-// Order by token: the place of row i is the number of rows with a smaller token, or the same
-// token and a smaller index.
-__global__ void __launch_bounds__(256) rank_kernel(const long* tokens, long V, long padding,
-                                                   unsigned* key, unsigned* order, int R) {
-    __shared__ unsigned ks[256];
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    auto key_of = [&](int j) {
-        const long t = tokens[j];
-        return t < 0 || t >= V || t == padding ? static_cast<unsigned>(V) : static_cast<unsigned>(t);
-    };
-    const unsigned mine = i < R ? key_of(i) : 0u;
-    int place = 0;
-    for (int j0 = 0; j0 < R; j0 += 256) {
-        __syncthreads();
-        if (j0 + static_cast<int>(threadIdx.x) < R) ks[threadIdx.x] = key_of(j0 + threadIdx.x);
-        __syncthreads();
-        const int m = R - j0 < 256 ? R - j0 : 256;
-        for (int j = 0; j < m; ++j) place += ks[j] < mine || (ks[j] == mine && j0 + j < i);
-    }
-    if (i < R) {
-        key[place] = mine;
-        order[place] = static_cast<unsigned>(i);
-    }
+// ---------------------------------------------------------------------------------------------
+// Order by token.  A token without a gradient (outside the table, padding) has the key V.
+__device__ __forceinline__ unsigned key_of(const long* tokens, long i, unsigned V, long padding) {
+    const long t = tokens[i];
+    return t < 0 || t >= static_cast<long>(V) || t == padding ? V : static_cast<unsigned>(t);
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) zero_kernel(T* p, long n) {
-    for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < n;
-         i += static_cast<long>(gridDim.x) * 256)
-        p[i] = static_cast<T>(0.f);
-}
+// Few tokens, one launch: the place of row i is the number of rows with a smaller key, or the
+// same key and a smaller index.  A workgroup places 64 rows, its 16 waves each count one
+// sixteenth of the keys; the keys counted are the same for all lanes, so they come by scalar
+// loads and cost two vector instructions each.
+constexpr int kRankWaves = 16;
 
-// One wave per sorted position and 512 columns; the first position of a run sums it.
-template <class T, class G>
-__global__ void __launch_bounds__(256) embedding_bwd_kernel(const unsigned* key, const unsigned* order,
-                                                            const T* dx, G* dw, int R, long V, long C,
-                                                            int slabs, float scale, int accumulate,
-                                                            DropRows d) {
-    const int lane = threadIdx.x & 63;
-    const long w = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int i = static_cast<int>(w / slabs);
-    if (i >= R) return;
-    const unsigned k = key[i];
-    if (k >= static_cast<unsigned>(V) || (i > 0 && key[i - 1] == k)) return;
-    const long c = (w % slabs) * 512 + lane * 8;
-    if (c >= C) return;
-    const int n = C - c >= 8 ? 8 : static_cast<int>(C - c);
-    const unsigned step = drop_step(d);
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int j = i; j < R && key[j] == k; ++j) {
-        const long r = order[j];
-        if (r >= R) continue;  // (no row: an order that is not of these tokens)
-        float f[8];
-        load_unit(dx + r * C + c, n, f);
-        if (d.limit != 0) drop8(d, step, d.first + r * C + c, f);
+__global__ void __launch_bounds__(64 * kRankWaves) rank_kernel(const long* tokens, unsigned V, long padding,
+                                                               unsigned* key, unsigned* order, int R) {
+    __shared__ unsigned count[kRankWaves][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i0 = blockIdx.x * 64, i = i0 + lane;
+    const unsigned mine = i < R ? key_of(tokens, i, V, padding) : 0u;
+    const int per = (R + kRankWaves - 1) / kRankWaves;
+    const int lo = min(R, wave * per), hi = min(R, lo + per);
+    unsigned n = 0;
+    int j = lo;
+    // an equal key counts where its row comes first
+    for (const int end = min(hi, i0); j < end; ++j) n += key_of(tokens, j, V, padding) <= mine;
+    for (const int end = min(hi, i0 + 64); j < end; ++j) {
+        const unsigned k = key_of(tokens, j, V, padding);
+        n += k < mine || (k == mine && j < i);
+    }
+    for (; j < hi; ++j) n += key_of(tokens, j, V, padding) < mine;
+    count[wave][lane] = n;
+    __syncthreads();
+    if (wave != 0 || i >= R) return;
+    unsigned place = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += f[q];
+    for (int w = 0; w < kRankWaves; ++w) place += count[w][lane];
+    key[place] = mine;
+    order[place] = static_cast<unsigned>(i);
+}
+
+// Many tokens: stable counting sort by 8 bits at a time, lowest first.  A tile is 2048 keys, four
+// waves with 512 consecutive keys each.
+constexpr int kTile = 2048, kDigits = 256;
+
+__device__ __forceinline__ unsigned tile_key(const long* tokens, const unsigned* from, long i, unsigned V,
+                                             long padding) {
+    return tokens != nullptr ? key_of(tokens, i, V, padding) : from[i];
+}
+
+// count[digit][tile]
+__global__ void __launch_bounds__(256) digit_count_kernel(const long* tokens, const unsigned* from,
+                                                          unsigned V, long padding, unsigned* count,
+                                                          long R, int shift) {
+    __shared__ unsigned hist[kDigits];
+    hist[threadIdx.x] = 0;
+    __syncthreads();
+    for (int k = 0; k < kTile / 256; ++k) {
+        const long i = static_cast<long>(blockIdx.x) * kTile + k * 256 + threadIdx.x;
+        if (i < R) atomicAdd(&hist[(tile_key(tokens, from, i, V, padding) >> shift) & 255u], 1u);
     }
+    __syncthreads();
+    count[static_cast<long>(threadIdx.x) * gridDim.x + blockIdx.x] = hist[threadIdx.x];
+}
+
+// Running sums in place, one workgroup.
+__global__ void __launch_bounds__(1024) digit_scan_kernel(unsigned* count, long n) {
+    __shared__ unsigned sums[16];
+    __shared__ unsigned carry;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0) carry = 0;
+    __syncthreads();
+    for (long base = 0; base < n; base += 4096) {
+        unsigned v[4], t = 0;
+        const long at = base + threadIdx.x * 4L;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { v[k] = at + k < n ? count[at + k] : 0u; t += v[k]; }
+        unsigned x = t;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const unsigned y = __shfl_up(x, off, 64);
+            if (lane >= off) x += y;
+        }
+        if (lane == 63) sums[wave] = x;
+        __syncthreads();
+        unsigned before = carry;
+        for (int w = 0; w < wave; ++w) before += sums[w];
+        before += x - t;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (at + k < n) count[at + k] = before;
+            before += v[k];
+        }
+        __syncthreads();
+        if (threadIdx.x == 1023) carry = before;
+        __syncthreads();
+    }
+}
+
+// To their places.  Within a wave the keys go 64 at a time: lanes with the same digit are found
+// by eight ballots, a lane's rank is the number of them before it.
+__global__ void __launch_bounds__(256) digit_scatter_kernel(const long* tokens, const unsigned* from,
+                                                            const unsigned* from_order, unsigned V,
+                                                            long padding, const unsigned* start,
+                                                            unsigned* key, unsigned* order, long R,
+                                                            int shift) {
+    __shared__ unsigned next[4][kDigits];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long i0 = static_cast<long>(blockIdx.x) * kTile + wave * (kTile / 4);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) next[w][threadIdx.x] = 0;
+    __syncthreads();
+    unsigned k[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const long i = i0 + r * 64 + lane;
+        k[r] = i < R ? tile_key(tokens, from, i, V, padding) : 0u;
+        if (i < R) atomicAdd(&next[wave][(k[r] >> shift) & 255u], 1u);
+    }
+    __syncthreads();
+    {   // the wave's first place of every digit
+        unsigned at = start[static_cast<long>(threadIdx.x) * gridDim.x + blockIdx.x];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const unsigned n = next[w][threadIdx.x];
+            next[w][threadIdx.x] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const long i = i0 + r * 64 + lane;
+        const bool in = i < R;
+        const unsigned d = (k[r] >> shift) & 255u;
+        unsigned long same = __ballot(in);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const unsigned long ones = __ballot((d >> b) & 1u);
+            same &= (d >> b) & 1u ? ones : ~ones;
+        }
+        const unsigned long below = same & ((1UL << lane) - 1UL);
+        // (the LDS operations of a wave complete in order: every lane reads before the first
+        // lane of each digit writes)
+        const unsigned first = in ? next[wave][d] : 0u;
+        __builtin_amdgcn_wave_barrier();
+        if (in && below == 0) next[wave][d] = first + static_cast<unsigned>(__popcll(same));
+        __builtin_amdgcn_wave_barrier();
+        if (in) {
+            const unsigned at = first + static_cast<unsigned>(__popcll(below));
+            key[at] = k[r];
+            order[at] = from_order != nullptr ? from_order[i] : static_cast<unsigned>(i);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradients.  The sorted positions are cut into chunks of `chunk`; a wave sums one chunk over 512
+// columns.  A run of equal tokens that lies within the chunk goes straight to its row; of a run
+// that goes on, the chunk's part goes to head[chunk] (it began before) or tail[chunk] (it begins
+// here), and the join kernel adds tail[chunk] + head[chunk + 1] + ... in a fixed order.  So a
+// frequent token costs as many rows per wave as any other.
+//
+// The same launch holds the waves of the position gradient (one per position and 512 columns,
+// summing over the sequences) and the workgroups that zero the rows of absent tokens (64 rows
+// each, present ones found by a search in the sorted keys), so that every byte of the gradient is
+// written once.
+constexpr int kMaxChunk = 32;
+
+struct BwdArgs {
+    const unsigned *key, *order;
+    const void* dx;
+    void *dw, *dp;
+    float *head, *tail;   // [chunks][C]
+    long B, T, V, C;
+    int R, chunk, chunks, slabs, accumulate;
+    float scale;
+    unsigned sum_blocks, pos_blocks;  // workgroups of the first two kinds
+    DropRows d;
+};
+
+__device__ __forceinline__ void add8(float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] += b[i];
+}
+
+template <class G>
+__device__ __forceinline__ void write_row(const BwdArgs& a, unsigned k, long c, int n, float (&acc)[8]) {
+    G* row = static_cast<G*>(a.dw) + static_cast<long>(k) * a.C + c;
     float old[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (accumulate) load_unit(dw + k * C + c, n, old);
+    if (a.accumulate) load_unit(row, n, old);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) acc[q] = fmaf(acc[q], scale, old[q]);
-    store_unit(dw + k * C + c, n, acc);
+    for (int q = 0; q < 8; ++q) acc[q] = fmaf(acc[q], a.scale, old[q]);
+    store_unit(row, n, acc);
 }
 
 template <class T, class G>
-__global__ void __launch_bounds__(256) positions_bwd_kernel(const T* dx, G* dp, long B, long Tn, long C,
-                                                            int slabs, DropRows d) {
-    const int lane = threadIdx.x & 63;
-    const long w = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const long t = w / slabs;
-    const long c = (w % slabs) * 512 + lane * 8;
-    if (t >= Tn || c >= C) return;
-    const int n = C - c >= 8 ? 8 : static_cast<int>(C - c);
-    const unsigned step = drop_step(d);
+__device__ __forceinline__ void sum_chunk(const BwdArgs& a, long w, int lane) {
+    const int ch = static_cast<int>(w / a.slabs);
+    if (ch >= a.chunks) return;
+    const int p0 = ch * a.chunk, len = min(a.chunk, a.R - p0);
+    // lane l holds key and row of position p0 - 1 + l (one before, one behind the chunk)
+    const int p = p0 - 1 + lane;
+    const bool there = p >= 0 && p < a.R && lane <= len + 1;
+    const int kv = there ? static_cast<int>(a.key[p]) : -1, ov = there ? static_cast<int>(a.order[p]) : -1;
+    const long c = (w % a.slabs) * 512 + lane * 8;
+    const int n = a.C - c >= 8 ? 8 : static_cast<int>(a.C - c);  // <= 0: no columns
+    const unsigned step = drop_step(a.d);
+    const T* dx = static_cast<const T*>(a.dx);
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (long b = 0; b < B; ++b) {
-        const long e = (b * Tn + t) * C + c;
-        float f[8];
-        load_unit(dx + e, n, f);
-        if (d.limit != 0) drop8(d, step, d.first + e, f);
+    bool head = __builtin_amdgcn_readlane(kv, 0) == __builtin_amdgcn_readlane(kv, 1);
+    constexpr int kBatch = 4;  // rows in flight
+    for (int j0 = 0; j0 < len; j0 += kBatch) {
+        float f[kBatch][8];
+        long row[kBatch];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += f[q];
+        for (int q = 0; q < kBatch; ++q) {
+            row[q] = j0 + q < len ? __builtin_amdgcn_readlane(ov, 1 + j0 + q) : -1;
+            // (out of range: an order that is not of these tokens)
+            const bool ok = row[q] >= 0 && row[q] < a.R && n > 0;
+            if (ok) load_unit(dx + row[q] * a.C + c, n, f[q]);
+            if (!ok) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[q][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            if (j0 + q >= len) break;
+            const int k = __builtin_amdgcn_readlane(kv, 1 + j0 + q), after = __builtin_amdgcn_readlane(kv, 2 + j0 + q);
+            if (a.d.limit != 0 && row[q] >= 0) drop8(a.d, step, a.d.first + row[q] * a.C + c, f[q]);
+            add8(acc, f[q]);
+            const bool last = j0 + q + 1 == len;
+            if (k == after && !last) continue;
+            const bool known = k >= 0 && static_cast<unsigned>(k) < static_cast<unsigned>(a.V);
+            if (known && n > 0) {
+                if (head) store_unit(a.head + static_cast<long>(ch) * a.C + c, n, acc);
+                else if (k == after) store_unit(a.tail + static_cast<long>(ch) * a.C + c, n, acc);
+                else write_row<G>(a, static_cast<unsigned>(k), c, n, acc);
+            }
+            head = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+        }
     }
-    store_unit(dp + t * C + c, n, acc);
+}
+
+template <class T, class G>
+__device__ __forceinline__ void sum_position(const BwdArgs& a, long w, int lane) {
+    const long t = w / a.slabs, c = (w % a.slabs) * 512 + lane * 8;
+    if (t >= a.T || c >= a.C) return;
+    const int n = a.C - c >= 8 ? 8 : static_cast<int>(a.C - c);
+    const unsigned step = drop_step(a.d);
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (long b = 0; b < a.B; ++b) {
+        const long e = (b * a.T + t) * a.C + c;
+        float f[8];
+        load_unit(static_cast<const T*>(a.dx) + e, n, f);
+        if (a.d.limit != 0) drop8(a.d, step, a.d.first + e, f);
+        add8(acc, f);
+    }
+    store_unit(static_cast<G*>(a.dp) + t * a.C + c, n, acc);
+}
+
+template <class G>
+__device__ __forceinline__ void zero_absent(const BwdArgs& a, long block) {
+    const int lane = threadIdx.x & 63;
+    const long v = block * 64 + lane;
+    int lo = 0, hi = a.R;  // the first position whose key is at least v
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.key[mid] < static_cast<unsigned long>(v)) lo = mid + 1; else hi = mid;
+    }
+    unsigned long absent = __ballot(v < a.V && !(lo < a.R && a.key[lo] == static_cast<unsigned long>(v)));
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    while (absent != 0) {
+        const int r = __builtin_ctzl(absent);
+        absent &= absent - 1;
+        G* row = static_cast<G*>(a.dw) + (block * 64 + r) * a.C;
+        for (long c = threadIdx.x * 8L; c < a.C; c += 2048)
+            store_unit(row + c, a.C - c >= 8 ? 8 : static_cast<int>(a.C - c), zero);
+    }
+}
+
+template <class T, class G>
+__global__ void __launch_bounds__(256) embedding_bwd_kernel(BwdArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned block = blockIdx.x;
+    if (block < a.sum_blocks) sum_chunk<T, G>(a, block * 4L + wave, lane);
+    else if (block < a.sum_blocks + a.pos_blocks) sum_position<T, G>(a, (block - a.sum_blocks) * 4L + wave, lane);
+    else zero_absent<G>(a, block - a.sum_blocks - a.pos_blocks);
+}
+
+// One workgroup per chunk and 512 columns: where a run begins in the chunk and goes on, its waves
+// sum the parts of the chunks behind, every eighth each, and the first adds them up.
+template <class G>
+__global__ void __launch_bounds__(512) embedding_join_kernel(BwdArgs a) {
+    __shared__ float part[8][512];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ch = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
+    const int p0 = ch * a.chunk, pe = p0 + a.chunk;  // (the last chunk has no join)
+    if (pe >= a.R) return;
+    const unsigned k = a.key[pe];
+    if (a.key[pe - 1] != k || k >= static_cast<unsigned>(a.V)) return;
+    if (a.key[p0] == k && p0 > 0 && a.key[p0 - 1] == k) return;  // it began before the chunk
+    // chunks behind this one whose first key is k hold a part in head[]
+    int more = 0;
+    for (int c0 = ch + 1;; c0 += 64) {
+        const unsigned long same = __ballot(c0 + lane < a.chunks && a.key[static_cast<long>(c0 + lane) * a.chunk] == k);
+        more += __popcll(same);
+        if (same != ~0UL) break;
+    }
+    const long c = slab * 512L + lane * 8;
+    const int n = a.C - c >= 8 ? 8 : static_cast<int>(a.C - c);
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n > 0) {
+#pragma unroll 4
+        for (int m = wave; m < more; m += 8) {
+            float f[8];
+            load_unit(a.head + static_cast<long>(ch + 1 + m) * a.C + c, n, f);
+            add8(acc, f);
+        }
+    }
+    store8(&part[wave][lane * 8], acc);
+    __syncthreads();
+    if (wave != 0 || n <= 0) return;
+    load_unit(a.tail + static_cast<long>(ch) * a.C + c, n, acc);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        float f[8];
+        load8(&part[w][lane * 8], f);
+        add8(acc, f);
+    }
+    write_row<G>(a, k, c, n, acc);
 }
 
 inline DropRows drop_rows(unsigned limit, unsigned long long seed, const long* step_at, unsigned step,
@@ -155,20 +404,26 @@ int fwd(const long* tokens, const void* table, const void* pos, void* out, long 
     return 0;
 }
 
+// positions per chunk: enough chunks to fill the chip, up to 32 rows per wave
+int chunk_of(long R, int slabs) {
+    int chunk = kMaxChunk;
+    while (chunk > 4 && R * slabs / chunk < 2048) chunk >>= 1;
+    return chunk;
+}
+
 template <class T, class G>
-int bwd(const unsigned* key, const unsigned* order, const void* dx, void* dw, void* dp, long B, long Tn,
-        long V, long C, float scale, int accumulate, const DropRows& d, hipStream_t s) {
-    const int slabs = static_cast<int>((C + 511) / 512);
-    const long R = B * Tn;
-    if (!accumulate)
-        hipLaunchKernelGGL((zero_kernel<G>), dim3(4096), dim3(256), 0, s, static_cast<G*>(dw), V * C);
-    hipLaunchKernelGGL((embedding_bwd_kernel<T, G>), dim3(static_cast<unsigned>((R * slabs + 3) / 4)),
-                       dim3(256), 0, s, key, order, static_cast<const T*>(dx), static_cast<G*>(dw),
-                       static_cast<int>(R), V, C, slabs, scale, accumulate, d);
-    if (dp != nullptr)
-        hipLaunchKernelGGL((positions_bwd_kernel<T, G>), dim3(static_cast<unsigned>((Tn * slabs + 3) / 4)),
-                           dim3(256), 0, s, static_cast<const T*>(dx), static_cast<G*>(dp), B, Tn, C,
-                           slabs, d);
+int bwd(BwdArgs a, hipStream_t s) {
+    const long sum = (static_cast<long>(a.chunks) * a.slabs + 3) / 4;
+    const long pos = a.dp != nullptr ? (a.T * a.slabs + 3) / 4 : 0;
+    const long zero = a.accumulate ? 0 : (a.V + 63) / 64;
+    if (sum + pos + zero > kMaxBlocks) return -3;
+    a.sum_blocks = static_cast<unsigned>(sum);
+    a.pos_blocks = static_cast<unsigned>(pos);
+    hipLaunchKernelGGL((embedding_bwd_kernel<T, G>), dim3(static_cast<unsigned>(sum + pos + zero)), dim3(256),
+                       0, s, a);
+    if (a.chunks > 1)
+        hipLaunchKernelGGL((embedding_join_kernel<G>), dim3(static_cast<unsigned>(a.chunks) * a.slabs), dim3(512),
+                           0, s, a);
     return static_cast<int>(hipGetLastError());
 }
 
@@ -192,33 +447,80 @@ int nf_embedding_fwd(const long* tokens, const void* table, const void* pos, voi
     }
 }
 
+// Rows up to which the one-launch form is taken (it does R^2 comparisons).
+static const long kRankRows = 8192;
+
+// unsigned words of scratch that nf_token_order needs
+long nf_token_order_words(long R) {
+    return R <= kRankRows ? 0 : 2 * R + ((R + kTile - 1) / kTile) * kDigits;
+}
+
 // key[i]: the i-th smallest token (V: none, or the padding token), order[i]: its row; equal
 // tokens in the order of their rows.
-int nf_token_order(const long* tokens, unsigned* key, unsigned* order, long R, long V, long padding,
-                   hipStream_t s) {
+int nf_token_order(const long* tokens, unsigned* key, unsigned* order, unsigned* scratch, long R, long V,
+                   long padding, hipStream_t s) {
     if (R <= 0 || R >= (1L << 31) || V <= 0 || V >= (1L << 31)) return -1;
-    hipLaunchKernelGGL(rank_kernel, dim3(static_cast<unsigned>((R + 255) / 256)), dim3(256), 0, s,
-                       tokens, V, padding, key, order, static_cast<int>(R));
+    const unsigned v = static_cast<unsigned>(V);
+    if (R <= kRankRows) {
+        hipLaunchKernelGGL(rank_kernel, dim3(static_cast<unsigned>((R + 63) / 64)), dim3(64 * kRankWaves), 0, s,
+                           tokens, v, padding, key, order, static_cast<int>(R));
+        return static_cast<int>(hipGetLastError());
+    }
+    const long tiles = (R + kTile - 1) / kTile;
+    unsigned *other_key = scratch, *other_order = scratch + R, *count = scratch + 2 * R;
+    int passes = 1;
+    while (passes < 4 && (v >> (8 * passes)) != 0) ++passes;
+    const unsigned *from = nullptr, *from_order = nullptr;
+    const dim3 grid(static_cast<unsigned>(tiles));
+    for (int p = 0; p < passes; ++p) {
+        const bool last = (passes - p) & 1;  // the passes alternate, the last one ends in key / order
+        unsigned *to = last ? key : other_key, *to_order = last ? order : other_order;
+        const long* tok = p == 0 ? tokens : nullptr;
+        hipLaunchKernelGGL(digit_count_kernel, grid, dim3(256), 0, s, tok, from, v, padding, count, R, 8 * p);
+        hipLaunchKernelGGL(digit_scan_kernel, dim3(1), dim3(1024), 0, s, count, tiles * kDigits);
+        hipLaunchKernelGGL(digit_scatter_kernel, grid, dim3(256), 0, s, tok, from, from_order, v, padding, count,
+                           to, to_order, R, 8 * p);
+        from = to;
+        from_order = to_order;
+    }
     return static_cast<int>(hipGetLastError());
+}
+
+// floats of scratch that nf_embedding_bwd needs
+long nf_embedding_bwd_floats(long R, long C) {
+    const int chunk = chunk_of(R, static_cast<int>((C + 511) / 512));
+    return 2 * ((R + chunk - 1) / chunk) * C;
 }
 
 // key / order: from nf_token_order.  dx: B T rows of C.  dw [V][C]: written everywhere, or
 // (accumulate) added to where tokens are.  dp (may be null): rows 0 .. T - 1 are written.
 // type: of dx; grad_type: of dw and dp (0, or the type of dx).
 int nf_embedding_bwd(const unsigned* key, const unsigned* order, const void* dx, void* dw, void* dp,
-                     int type, int grad_type, long B, long T, long V, long C, float scale,
+                     float* scratch, int type, int grad_type, long B, long T, long V, long C, float scale,
                      int accumulate, unsigned limit, unsigned long long seed, const long* step_at,
                      unsigned step, long first, hipStream_t s) {
     if (B <= 0 || T <= 0 || V <= 0 || C <= 0 || limit > 65535u || first < 0) return -1;
-    if (B * T >= (1L << 31) || B * T * ((C + 511) / 512) >= (1L << 32)) return -3;
+    if (V >= (1L << 31) || C >= (1L << 24) || B >= (1L << 31) || T >= (1L << 31) || B * T >= (1L << 31)) return -3;
     if (grad_type != 0 && grad_type != type) return -1;
-    const DropRows d = drop_rows(limit, seed, step_at, step, first);
+    BwdArgs a = {};
+    a.key = key; a.order = order; a.dx = dx; a.dw = dw; a.dp = dp;
+    a.B = B; a.T = T; a.V = V; a.C = C;
+    a.R = static_cast<int>(B * T);
+    a.slabs = static_cast<int>((C + 511) / 512);
+    a.chunk = chunk_of(a.R, a.slabs);
+    a.chunks = static_cast<int>((a.R + static_cast<long>(a.chunk) - 1) / a.chunk);
+    a.head = scratch;
+    a.tail = scratch + static_cast<long>(a.chunks) * C;
+    a.accumulate = accumulate;
+    a.scale = scale;
+    a.d = drop_rows(limit, seed, step_at, step, first);
+    if (static_cast<long>(a.chunks) * a.slabs > (1L << 22)) return -3;
     switch (type * 4 + grad_type) {
-    case 0: return bwd<float, float>(key, order, dx, dw, dp, B, T, V, C, scale, accumulate, d, s);
-    case 4: return bwd<bf16, float>(key, order, dx, dw, dp, B, T, V, C, scale, accumulate, d, s);
-    case 5: return bwd<bf16, bf16>(key, order, dx, dw, dp, B, T, V, C, scale, accumulate, d, s);
-    case 8: return bwd<half, float>(key, order, dx, dw, dp, B, T, V, C, scale, accumulate, d, s);
-    case 10: return bwd<half, half>(key, order, dx, dw, dp, B, T, V, C, scale, accumulate, d, s);
+    case 0: return bwd<float, float>(a, s);
+    case 4: return bwd<bf16, float>(a, s);
+    case 5: return bwd<bf16, bf16>(a, s);
+    case 8: return bwd<half, float>(a, s);
+    case 10: return bwd<half, half>(a, s);
     default: return -1;
     }
 }

@@ -27,8 +27,10 @@ from .dropout import FLOAT_TYPES, check_key, kept_rows, limit_of, step_args
 P, L, I, U, UL, FL = c_void_p, c_long, c_int, c_uint, c_ulonglong, c_float
 _SIGS = {
     "nf_embedding_fwd": ([P, P, P, P, I, L, L, L, L, FL, U, UL, P, U, L, P], I),
-    "nf_token_order": ([P, P, P, L, L, L, P], I),
-    "nf_embedding_bwd": ([P, P, P, P, P, I, I, L, L, L, L, FL, I, U, UL, P, U, L, P], I),
+    "nf_token_order_words": ([L], L),
+    "nf_token_order": ([P, P, P, P, L, L, L, P], I),
+    "nf_embedding_bwd_floats": ([L, L], L),
+    "nf_embedding_bwd": ([P, P, P, P, P, P, I, I, L, L, L, L, FL, I, U, UL, P, U, L, P], I),
 }
 _fns: dict[str, object] = {}
 
@@ -137,9 +139,11 @@ def token_order(tokens: torch.Tensor, vocab: int, padding_idx: int | None = None
         return key.to(torch.int32), order.to(torch.int32)
     key, order = torch.empty(2, R, dtype=torch.int32, device=dev).unbind(0)
     if R:
+        words = _fn("nf_token_order_words")(R)
+        scratch = torch.empty(words, dtype=torch.int32, device=dev) if words else None
         with library.on_device(dev):
-            library.check(_fn("nf_token_order")(tokens.data_ptr(), key.data_ptr(), order.data_ptr(), R,
-                                                vocab, padding, library.stream_ptr(dev)), "token_order")
+            library.check(_fn("nf_token_order")(tokens.data_ptr(), key.data_ptr(), order.data_ptr(),
+                                                scratch.data_ptr() if words else None, R, vocab, padding, library.stream_ptr(dev)), "token_order")
     return key, order
 
 
@@ -200,9 +204,12 @@ def embedding_bwd(tokens: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor
         return
     key, rows = order if order is not None else token_order(tokens, V, padding_idx)
     at, number = step_args(step)
+    # (scratch of its own for every call: the allocator hands it on in stream order, and a captured
+    # call's belongs to its graph)
+    scratch = torch.empty(_fn("nf_embedding_bwd_floats")(R, C), dtype=torch.float32, device=dev)
     with library.on_device(dev):
         library.check(_fn("nf_embedding_bwd")(
             key.data_ptr(), rows.data_ptr(), dout.data_ptr(), dtable.data_ptr(),
-            dpositions.data_ptr() if dpositions is not None else None, FLOAT_TYPES[dout.dtype],
-            FLOAT_TYPES[dtable.dtype], B, T, V, C, scale, int(accumulate), limit, seed, at, number,
+            dpositions.data_ptr() if dpositions is not None else None, scratch.data_ptr(),
+            FLOAT_TYPES[dout.dtype], FLOAT_TYPES[dtable.dtype], B, T, V, C, scale, int(accumulate), limit, seed, at, number,
             first, library.stream_ptr(dev)), "embedding_bwd")

@@ -82,6 +82,8 @@ struct AttnArgs {
     int B, Tq, Tk, H, Hk, D, causal;
     float scale, up;
     unsigned limit, step;
+    float* parts;             // few queries: partial results of the key chunks, or null (one chunk)
+    int chunk;                // keys per chunk
 };
 
 // -- tiles ------------------------------------------------------------------------------------
@@ -403,6 +405,242 @@ attn_fwd_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// Forward of few queries (queries x heads per key head <= 32) against many keys: the queries of
+// all heads that share a key head are the columns of one tile, so the keys are read once for all
+// of them.  Bound by reading the keys and values.  A workgroup takes a chunk of the keys (grid =
+// sequence and key head, chunk), its waves every fourth 32 of them; a wave reads K straight into
+// operand fragments and V through LDS of its own (no barrier in the loop), one tile ahead.  The
+// waves are joined through LDS, the chunks by attn_join_kernel.
+constexpr int kFew = 32;
+
+// parts: [B Hk][chunks][rows][DP] of O, then [B Hk][chunks][rows] x (m, l)
+template <class E, int DP>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+attn_few_kernel(AttnArgs a) {
+    typedef Tile<E, DP, 32> T;
+    typedef typename T::x8 x8;
+    constexpr int NB = DP / 32, KS = DP / 16, kVPer = 32 * T::kPieces / 64;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int bh = blockIdx.x, b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
+    const int lane = threadIdx.x & 63, n = lane & 31, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Seq sq = sequence(a, b);
+    const int rows = a.Tq * group, qi = n / group, h = hk * group + n % group;
+    const bool in = n < rows && qi < sq.m;
+    const int seen = (in ? keys_seen(sq, qi) : 0) - 4 * hh;
+    const int k0 = blockIdx.y * a.chunk, k1 = min(sq.m > 0 ? sq.n : 0, k0 + a.chunk);
+    char* lds = smem + wave * T::kBytes;
+    const typename T::Lane at = T::lane_offsets(lane);
+    x8 qf[KS];
+    own_row<E, DP>(static_cast<const E*>(a.q) + b * a.sq.b + qi * a.sq.t + h * a.sq.h, in, a.D, hh, qf);
+    unsigned koff[KS], voff[kVPer];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int c = ks * 16 + 8 * hh;
+        koff[ks] = c < a.D ? static_cast<unsigned>(n * a.sk.t + c) * 2u : 0x80000000u;
+    }
+#pragma unroll
+    for (int i = 0; i < kVPer; ++i) {
+        const int idx = lane + 64 * i, c = (idx % T::kPieces) * 8;
+        voff[i] = c < a.D ? static_cast<unsigned>((idx / T::kPieces) * a.sv.t + c) * 2u : 0x80000000u;
+    }
+    const E* kb = static_cast<const E*>(a.k) + b * a.sk.b + hk * a.sk.h;
+    const E* vb = static_cast<const E*>(a.v) + b * a.sv.b + hk * a.sv.h;
+    u32x4 kr[KS], vr[kVPer];
+    auto fetch = [&](int key0) {  // rows behind the last key read as 0
+        const long last = min(sq.n - key0, 32) - 1;
+        const __amdgpu_buffer_rsrc_t kd = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<E*>(kb + key0 * a.sk.t), 0, static_cast<int>((last * a.sk.t + a.D) * 2), 0x00020000);
+        const __amdgpu_buffer_rsrc_t vd = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<E*>(vb + key0 * a.sv.t), 0, static_cast<int>((last * a.sv.t + a.D) * 2), 0x00020000);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            kr[ks] = __builtin_amdgcn_raw_buffer_load_b128(kd, static_cast<int>(koff[ks]), 0, 0);
+#pragma unroll
+        for (int i = 0; i < kVPer; ++i)
+            vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vd, static_cast<int>(voff[i]), 0, 0);
+    };
+    f32x16 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o[i] = f32x16{0};
+    float m = -INFINITY, l = 0.f, msc = 0.f;
+    const float sc2 = a.scale * kLog2e;
+    int key0 = k0 + wave * 32;
+    if (key0 < k1) fetch(key0);
+    for (; key0 < k1; key0 += 128) {
+        f32x16 s = {0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = mma(__builtin_bit_cast(x8, kr[ks]), qf[ks], s);
+        // (the LDS operations of a wave complete in order: the reads of the tile before come first)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < kVPer; ++i) {
+            const int idx = lane + 64 * i;
+            *reinterpret_cast<u32x4*>(lds + nfix::attn_off(DP, idx / T::kPieces, idx % T::kPieces)) = vr[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (key0 + 128 < k1) fetch(key0 + 128);
+        const int lim = min(seen, k1 - 4 * hh) - key0;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (reg_row(r) >= lim) s[r] = -INFINITY;
+            mx = fmaxf(mx, s[r]);
+        }
+        mx = max_halves(mx);
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            const float alpha = exp2_fast((m - ref) * sc2);
+            m = mn;
+            msc = ref * sc2;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+        }
+        float rs = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = exp2_fast(fmaf(s[r], sc2, -msc));
+            rs += s[r];
+        }
+        l += rs;
+        const x8 p0 = pack8<E>(s, 0), p1 = pack8<E>(s, 8);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            o[i] = mma(T::tr(lds, at, 0, i), p0, o[i]);
+            o[i] = mma(T::tr(lds, at, 16, i), p1, o[i]);
+        }
+    }
+    l = sum_halves(l);
+    // join the waves: 2, 3 into 0, 1, then 1 into 0
+    constexpr int kPark = 64 * (NB * 16 + 2);
+    float* park = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+            float* to = park + (wave - half) * kPark + lane;
+            to[0] = m;
+            to[64] = l;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) to[64 * (2 + 16 * i + r)] = o[i][r];
+        }
+        __syncthreads();
+        if (wave < half) {
+            const float* from = park + wave * kPark + lane;
+            const float m2 = from[0], l2 = from[64], mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+            const float a1 = exp2_fast((m - ref) * sc2), a2 = exp2_fast((m2 - ref) * sc2);
+            m = mn;
+            l = l * a1 + l2 * a2;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] = o[i][r] * a1 + from[64 * (2 + 16 * i + r)] * a2;
+        }
+    }
+    if (wave != 0 || n >= rows) return;
+    if (a.parts != nullptr) {
+        const long part = (static_cast<long>(bh) * gridDim.y + blockIdx.y) * rows + n;
+        const long parts = static_cast<long>(gridDim.x) * gridDim.y * rows;
+        if (k0 >= k1) return;  // (a chunk without keys is not read)
+        if (hh == 0) {
+            a.parts[parts * DP + 2 * part] = m;
+            a.parts[parts * DP + 2 * part + 1] = l;
+        }
+        float* to = a.parts + part * DP;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = o[i][4 * g + e];
+                *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * hh) = v;
+            }
+        return;
+    }
+    const bool some = in && (l > 0.f || l != l);
+    const float inv = some ? 1.f / l : 0.f;
+    E* orow = static_cast<E*>(a.out) + b * a.so.b + qi * a.so.t + h * a.so.h;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            typename T::x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(some ? o[i][4 * g + e] * inv : 0.f);
+            const int c = 32 * i + 8 * g + 4 * hh;
+            if (c < a.D) *reinterpret_cast<typename T::x4*>(orow + c) = v;
+        }
+    if (hh == 0)
+        a.lse[(static_cast<long>(b) * a.H + h) * a.Tq + qi] =
+            some ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+}
+
+// One wave per row: the chunks' maxima and sums, 64 at a time, then their O in order.
+template <class E, int DP>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int chunks) {
+    const int lane = threadIdx.x & 63, group = a.H / a.Hk, rows = a.Tq * group;
+    const long row = static_cast<long>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long parts = static_cast<long>(a.B) * a.Hk * chunks * rows;
+    if (row >= static_cast<long>(a.B) * a.Hk * rows) return;
+    const long bh = row / rows;
+    const int r = static_cast<int>(row % rows), b = static_cast<int>(bh / a.Hk), hk = static_cast<int>(bh % a.Hk);
+    const int qi = r / group, h = hk * group + r % group;
+    const Seq sq = sequence(a, b);
+    const int live = qi < sq.m ? (sq.n + a.chunk - 1) / a.chunk : 0;
+    const float sc2 = a.scale * kLog2e;
+    const float* ml = a.parts + parts * DP;
+    float m = -INFINITY;
+    for (int c = lane; c < live; c += 64) m = fmaxf(m, ml[2 * ((bh * chunks + c) * rows + r)]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int c0 = 0; c0 < live; c0 += 64) {
+        float w = 0.f;
+        if (c0 + lane < live) {
+            const long p = (bh * chunks + c0 + lane) * rows + r;
+            w = exp2_fast((ml[2 * p] - ref) * sc2);
+            l = fmaf(ml[2 * p + 1], w, l);
+        }
+        const int more = min(64, live - c0);
+        const float* o = a.parts + ((bh * chunks + c0) * rows + r) * static_cast<long>(DP);
+        for (int c1 = 0; c1 < more; c1 += 8) {  // eight parts in flight
+            float v0[8], v1[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float* oc = o + min(c1 + u, more - 1) * static_cast<long>(rows) * DP;
+                v0[u] = oc[lane];
+                if (DP > 64) v1[u] = oc[64 + lane];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(c1 + u, 63)));
+                if (c1 + u < more) {
+                    o0 = fmaf(v0[u], wc, o0);
+                    if (DP > 64) o1 = fmaf(v1[u], wc, o1);
+                }
+            }
+        }
+    }
+    l = wave_sum(l);
+    const bool some = l > 0.f || l != l;
+    const float inv = some ? 1.f / l : 0.f;
+    E* orow = static_cast<E*>(a.out) + b * a.so.b + qi * a.so.t + h * a.so.h;
+    if (lane < a.D) orow[lane] = static_cast<E>(some ? o0 * inv : 0.f);
+    if (DP > 64 && 64 + lane < a.D) orow[64 + lane] = static_cast<E>(some ? o1 * inv : 0.f);
+    if (lane == 0)
+        a.lse[(static_cast<long>(b) * a.H + h) * a.Tq + qi] =
+            some ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------
 // Backward, queries: one workgroup = 128 queries; streams K / V.
 //
 // D = rowsum(dO * O) takes O as it was stored: rounded, and summed from rounded probabilities.
@@ -700,6 +938,33 @@ int launch_fwd(const AttnArgs& a, hipStream_t s) {
     return static_cast<int>(hipGetLastError());
 }
 
+// Keys per chunk of attn_few_kernel: about 1024 workgroups where the keys suffice, 128 keys (one
+// tile per wave) at least.  0: not the few-query form.
+int few_chunk(const AttnArgs& a) {
+    if (a.limit != 0 || static_cast<long>(a.Tq) * (a.H / a.Hk) > kFew) return 0;
+    const long per = (static_cast<long>(a.Tk) * a.B * a.Hk + 1023) / 1024;
+    const long chunk = per < 128 ? 128 : (per + 127) / 128 * 128;
+    return static_cast<int>(chunk < a.Tk ? chunk : (a.Tk + 127) / 128 * 128);
+}
+int few_chunks(const AttnArgs& a, int chunk) { return (a.Tk + chunk - 1) / chunk; }
+int padded_dim(int D) { return D <= 64 ? 64 : 128; }
+
+template <class E, int DP>
+int launch_few(AttnArgs a, hipStream_t s) {
+    constexpr int park = 2 * 64 * (DP / 32 * 16 + 2) * 4, v = 4 * Tile<E, DP, 32>::kBytes, lds = park > v ? park : v;
+    const int chunks = few_chunks(a, a.chunk);
+    if (chunks > 1 && a.parts == nullptr) return -2;
+    if (chunks == 1) a.parts = nullptr;
+    if (const int st = set_lds(reinterpret_cast<const void*>(attn_few_kernel<E, DP>), lds)) return st;
+    hipLaunchKernelGGL((attn_few_kernel<E, DP>), dim3(a.B * a.Hk, chunks), dim3(256), lds, s, a);
+    if (chunks > 1) {
+        const long rows = static_cast<long>(a.B) * a.H * a.Tq;
+        hipLaunchKernelGGL((attn_join_kernel<E, DP>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a,
+                           chunks);
+    }
+    return static_cast<int>(hipGetLastError());
+}
+
 template <class E, int DP, bool kDrop>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {
     constexpr int rows = kBwdStage<DP>;
@@ -714,6 +979,7 @@ int launch_bwd(const AttnArgs& a, hipStream_t s) {
 template <class E, int DP>
 int launch(const AttnArgs& a, int backward, hipStream_t s) {
     if (backward) return a.limit ? launch_bwd<E, DP, true>(a, s) : launch_bwd<E, DP, false>(a, s);
+    if (a.chunk != 0) return launch_few<E, DP>(a, s);
     return a.limit ? launch_fwd<E, DP, true>(a, s) : launch_fwd<E, DP, false>(a, s);
 }
 
@@ -728,10 +994,19 @@ extern "C" {
 
 int nf_attention_args_size() { return static_cast<int>(sizeof(AttnArgs)); }
 
+// floats of scratch that a forward call needs (args->parts)
+long nf_attention_fwd_floats(const AttnArgs* args) {
+    const AttnArgs& a = *args;
+    if (a.Hk <= 0 || a.Tk <= 0) return 0;
+    const int chunk = few_chunk(a);
+    if (chunk == 0 || few_chunks(a, chunk) == 1) return 0;
+    return static_cast<long>(a.B) * a.H * a.Tq * few_chunks(a, chunk) * (2 + padded_dim(a.D));
+}
+
 // type: 1 bf16, 2 half.  backward 0: reads q, k, v and writes out, lse; 1: reads q, k, v, out,
 // lse, dout and writes dq, dk, dv (delta: B H Tq floats of scratch).
 int nf_attention(const AttnArgs* args, int type, int backward, hipStream_t s) {
-    const AttnArgs& a = *args;
+    AttnArgs a = *args;
     if (a.B <= 0 || a.H <= 0 || a.Hk <= 0 || a.Tq <= 0 || a.Tk <= 0 || a.H % a.Hk != 0) return -1;
     if (a.D <= 0 || a.D > 128 || a.D % 8 != 0 || a.limit > 255u || !(a.scale > 0.f)) return -1;
     if (a.Tq > (1 << 22) || a.Tk > (1 << 22) || static_cast<long>(a.B) * a.H > (1 << 23)) return -3;
@@ -740,6 +1015,8 @@ int nf_attention(const AttnArgs* args, int type, int backward, hipStream_t s) {
     if (backward && (!fits(a.dout, a.sdo) || !fits(a.dq, a.sdq) || !fits(a.dk, a.sdk) ||
                      !fits(a.dv, a.sdv) || a.delta == nullptr))
         return -2;
+    a.chunk = backward ? 0 : few_chunk(a);
+    if (a.chunk != 0 && few_chunks(a, a.chunk) > 65535) return -3;
     if (type == 1) return a.D <= 64 ? launch<bf16, 64>(a, backward, s) : launch<bf16, 128>(a, backward, s);
     if (type == 2) return a.D <= 64 ? launch<half, 64>(a, backward, s) : launch<half, 128>(a, backward, s);
     return -1;

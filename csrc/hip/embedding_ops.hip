@@ -56,28 +56,41 @@ __device__ __forceinline__ unsigned key_of(const long* tokens, long i, unsigned 
 }
 
 // Few tokens, one launch: the place of row i is the number of rows with a smaller key, or the
-// same key and a smaller index.  A workgroup places 64 rows, its 16 waves each count one
-// sixteenth of the keys; the keys counted are the same for all lanes, so they come by scalar
-// loads and cost two vector instructions each.
-constexpr int kRankWaves = 16;
+// same key and a smaller index.  A workgroup holds all keys in LDS and places 64 rows, its 16
+// waves each count one sixteenth of the keys, four per (broadcast) LDS read and two vector
+// instructions each.
+constexpr int kRankWaves = 16, kRankRows = 8192;
 
 __global__ void __launch_bounds__(64 * kRankWaves) rank_kernel(const long* tokens, unsigned V, long padding,
                                                                unsigned* key, unsigned* order, int R) {
+    __shared__ __attribute__((aligned(16))) unsigned keys[kRankRows];
     __shared__ unsigned count[kRankWaves][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i0 = blockIdx.x * 64, i = i0 + lane;
-    const unsigned mine = i < R ? key_of(tokens, i, V, padding) : 0u;
-    const int per = (R + kRankWaves - 1) / kRankWaves;
-    const int lo = min(R, wave * per), hi = min(R, lo + per);
+    const int i0 = blockIdx.x * 64, i = i0 + lane, padded = (R + 63) & ~63;
+    // (behind the last row: keys that no row is behind)
+    for (int j = threadIdx.x; j < padded; j += 64 * kRankWaves)
+        keys[j] = j < R ? key_of(tokens, j, V, padding) : 0xFFFFFFFFu;
+    __syncthreads();
+    const unsigned mine = keys[i];  // (i < padded)
+    // 64 keys at a time; equal ones count where their row comes first
     unsigned n = 0;
-    int j = lo;
-    // an equal key counts where its row comes first
-    for (const int end = min(hi, i0); j < end; ++j) n += key_of(tokens, j, V, padding) <= mine;
-    for (const int end = min(hi, i0 + 64); j < end; ++j) {
-        const unsigned k = key_of(tokens, j, V, padding);
-        n += k < mine || (k == mine && j < i);
+    for (int j0 = wave * 64; j0 < padded; j0 += 64 * kRankWaves) {
+        if (j0 == i0) {
+            for (int j = 0; j < 64; ++j) {
+                const unsigned k = keys[j0 + j];
+                n += k < mine || (k == mine && j < lane);
+            }
+            continue;
+        }
+        const unsigned limit = j0 < i0 ? mine : mine - 1;  // count keys <= limit
+        const bool none = j0 > i0 && mine == 0;
+#pragma unroll
+        for (int j = 0; j < 64; j += 4) {
+            const uint4 k = *reinterpret_cast<const uint4*>(&keys[j0 + j]);
+            n += (k.x <= limit) + (k.y <= limit) + (k.z <= limit) + (k.w <= limit);
+        }
+        if (none) n -= 64;  // (mine - 1 wrapped: every key counted)
     }
-    for (; j < hi; ++j) n += key_of(tokens, j, V, padding) < mine;
     count[wave][lane] = n;
     __syncthreads();
     if (wave != 0 || i >= R) return;
@@ -88,100 +101,82 @@ __global__ void __launch_bounds__(64 * kRankWaves) rank_kernel(const long* token
     order[place] = static_cast<unsigned>(i);
 }
 
-// Many tokens: stable counting sort by 8 bits at a time, lowest first.  A tile is 2048 keys, four
-// waves with 512 consecutive keys each.
-constexpr int kTile = 2048, kDigits = 256;
+// Many tokens: stable counting sort by 8 bits at a time, lowest first, in two launches each: the
+// digits of every tile are counted, then every workgroup finds its own first places from all
+// counts and moves its tile.  A tile is 256 * rounds keys, four waves with 64 * rounds consecutive
+// ones each; with at most 128 tiles the counts are 128 rows of 1 KiB that every workgroup can
+// read for itself, which is cheaper than a launch for their running sums.
+constexpr int kDigits = 256, kMaxTiles = 128;
 
 __device__ __forceinline__ unsigned tile_key(const long* tokens, const unsigned* from, long i, unsigned V,
                                              long padding) {
     return tokens != nullptr ? key_of(tokens, i, V, padding) : from[i];
 }
 
-// count[digit][tile]
+// count[tile][digit]
 __global__ void __launch_bounds__(256) digit_count_kernel(const long* tokens, const unsigned* from,
                                                           unsigned V, long padding, unsigned* count,
-                                                          long R, int shift) {
+                                                          long R, int rounds, int shift) {
     __shared__ unsigned hist[kDigits];
     hist[threadIdx.x] = 0;
     __syncthreads();
-    for (int k = 0; k < kTile / 256; ++k) {
-        const long i = static_cast<long>(blockIdx.x) * kTile + k * 256 + threadIdx.x;
+    const long i0 = static_cast<long>(blockIdx.x) * rounds * 256;
+    for (int k = 0; k < rounds; ++k) {
+        const long i = i0 + k * 256 + threadIdx.x;
         if (i < R) atomicAdd(&hist[(tile_key(tokens, from, i, V, padding) >> shift) & 255u], 1u);
     }
     __syncthreads();
-    count[static_cast<long>(threadIdx.x) * gridDim.x + blockIdx.x] = hist[threadIdx.x];
+    count[blockIdx.x * kDigits + threadIdx.x] = hist[threadIdx.x];
 }
 
-// Running sums in place, one workgroup.
-__global__ void __launch_bounds__(1024) digit_scan_kernel(unsigned* count, long n) {
-    __shared__ unsigned sums[16];
-    __shared__ unsigned carry;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) carry = 0;
-    __syncthreads();
-    for (long base = 0; base < n; base += 4096) {
-        unsigned v[4], t = 0;
-        const long at = base + threadIdx.x * 4L;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { v[k] = at + k < n ? count[at + k] : 0u; t += v[k]; }
-        unsigned x = t;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const unsigned y = __shfl_up(x, off, 64);
-            if (lane >= off) x += y;
-        }
-        if (lane == 63) sums[wave] = x;
-        __syncthreads();
-        unsigned before = carry;
-        for (int w = 0; w < wave; ++w) before += sums[w];
-        before += x - t;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (at + k < n) count[at + k] = before;
-            before += v[k];
-        }
-        __syncthreads();
-        if (threadIdx.x == 1023) carry = before;
-        __syncthreads();
-    }
-}
-
-// To their places.  Within a wave the keys go 64 at a time: lanes with the same digit are found
-// by eight ballots, a lane's rank is the number of them before it.
-__global__ void __launch_bounds__(256) digit_scatter_kernel(const long* tokens, const unsigned* from,
-                                                            const unsigned* from_order, unsigned V,
-                                                            long padding, const unsigned* start,
-                                                            unsigned* key, unsigned* order, long R,
-                                                            int shift) {
+// Within a wave the keys go 64 at a time: lanes with the same digit are found by eight ballots, a
+// lane's rank is the number of them before it.
+__global__ void __launch_bounds__(256) digit_move_kernel(const long* tokens, const unsigned* from,
+                                                         const unsigned* from_order, unsigned V,
+                                                         long padding, const unsigned* count,
+                                                         unsigned* key, unsigned* order, long R,
+                                                         int rounds, int shift) {
     __shared__ unsigned next[4][kDigits];
+    __shared__ unsigned sums[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long i0 = static_cast<long>(blockIdx.x) * kTile + wave * (kTile / 4);
+    const long i0 = (static_cast<long>(blockIdx.x) * 4 + wave) * rounds * 64;
 #pragma unroll
     for (int w = 0; w < 4; ++w) next[w][threadIdx.x] = 0;
     __syncthreads();
-    unsigned k[8];
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < rounds; ++r) {
         const long i = i0 + r * 64 + lane;
-        k[r] = i < R ? tile_key(tokens, from, i, V, padding) : 0u;
-        if (i < R) atomicAdd(&next[wave][(k[r] >> shift) & 255u], 1u);
+        if (i < R) atomicAdd(&next[wave][(tile_key(tokens, from, i, V, padding) >> shift) & 255u], 1u);
+    }
+    // thread d: keys with digit d in the tiles before this one, and in all
+    unsigned before = 0, all = 0;
+    const int tiles = gridDim.x, mine = blockIdx.x;
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) {
+        const unsigned n = count[t * kDigits + threadIdx.x];
+        before += t < mine ? n : 0u;
+        all += n;
+    }
+    unsigned x = all;  // running sum over the digits
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const unsigned y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+    }
+    if (lane == 63) sums[wave] = x;
+    __syncthreads();
+    unsigned at = before + x - all;
+    for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {  // every wave's first place of digit threadIdx.x
+        const unsigned n = next[w][threadIdx.x];
+        next[w][threadIdx.x] = at;
+        at += n;
     }
     __syncthreads();
-    {   // the wave's first place of every digit
-        unsigned at = start[static_cast<long>(threadIdx.x) * gridDim.x + blockIdx.x];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const unsigned n = next[w][threadIdx.x];
-            next[w][threadIdx.x] = at;
-            at += n;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < rounds; ++r) {
         const long i = i0 + r * 64 + lane;
         const bool in = i < R;
-        const unsigned d = (k[r] >> shift) & 255u;
+        const unsigned k = in ? tile_key(tokens, from, i, V, padding) : 0u, d = (k >> shift) & 255u;
         unsigned long same = __ballot(in);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
@@ -189,16 +184,16 @@ __global__ void __launch_bounds__(256) digit_scatter_kernel(const long* tokens, 
             same &= (d >> b) & 1u ? ones : ~ones;
         }
         const unsigned long below = same & ((1UL << lane) - 1UL);
-        // (the LDS operations of a wave complete in order: every lane reads before the first
-        // lane of each digit writes)
+        // (the LDS operations of a wave complete in order: every lane reads before the first lane
+        // of each digit writes)
         const unsigned first = in ? next[wave][d] : 0u;
-        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (in && below == 0) next[wave][d] = first + static_cast<unsigned>(__popcll(same));
-        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (in) {
-            const unsigned at = first + static_cast<unsigned>(__popcll(below));
-            key[at] = k[r];
-            order[at] = from_order != nullptr ? from_order[i] : static_cast<unsigned>(i);
+            const unsigned place = first + static_cast<unsigned>(__popcll(below));
+            key[place] = k;
+            order[place] = from_order != nullptr ? from_order[i] : static_cast<unsigned>(i);
         }
     }
 }
@@ -321,14 +316,20 @@ __device__ __forceinline__ void zero_absent(const BwdArgs& a, long block) {
         const int mid = (lo + hi) >> 1;
         if (a.key[mid] < static_cast<unsigned long>(v)) lo = mid + 1; else hi = mid;
     }
-    unsigned long absent = __ballot(v < a.V && !(lo < a.R && a.key[lo] == static_cast<unsigned long>(v)));
+    const unsigned long absent = __ballot(v < a.V && !(lo < a.R && a.key[lo] == static_cast<unsigned long>(v)));
+    // the 64 rows are one stretch of memory, walked in (aligned) units of eight whatever the row length
     const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    while (absent != 0) {
-        const int r = __builtin_ctzl(absent);
-        absent &= absent - 1;
-        G* row = static_cast<G*>(a.dw) + (block * 64 + r) * a.C;
-        for (long c = threadIdx.x * 8L; c < a.C; c += 2048)
-            store_unit(row + c, a.C - c >= 8 ? 8 : static_cast<int>(a.C - c), zero);
+    const unsigned C = static_cast<unsigned>(a.C), n = static_cast<unsigned>(min(64L, a.V - block * 64)) * C;
+    G* rows = static_cast<G*>(a.dw) + block * 64 * a.C;
+    for (unsigned e = threadIdx.x * 8; e < n; e += 2048) {
+        const unsigned r = e / C, end = min(e + 8, n);
+        const unsigned long bits = absent >> r;
+        if (end == e + 8 && (bits & 1) && ((r + 1) * C >= end || ((bits & 2) && (r + 2) * C >= end))) {
+            store8(rows + e, zero);
+        } else {
+            for (unsigned i = e; i < end; ++i)
+                if ((absent >> (i / C)) & 1) rows[i] = static_cast<G>(0.f);
+        }
     }
 }
 
@@ -447,12 +448,9 @@ int nf_embedding_fwd(const long* tokens, const void* table, const void* pos, voi
     }
 }
 
-// Rows up to which the one-launch form is taken (it does R^2 comparisons).
-static const long kRankRows = 8192;
-
 // unsigned words of scratch that nf_token_order needs
 long nf_token_order_words(long R) {
-    return R <= kRankRows ? 0 : 2 * R + ((R + kTile - 1) / kTile) * kDigits;
+    return R <= kRankRows ? 0 : 2 * R + kMaxTiles * kDigits;
 }
 
 // key[i]: the i-th smallest token (V: none, or the padding token), order[i]: its row; equal
@@ -466,44 +464,43 @@ int nf_token_order(const long* tokens, unsigned* key, unsigned* order, unsigned*
                            tokens, v, padding, key, order, static_cast<int>(R));
         return static_cast<int>(hipGetLastError());
     }
-    const long tiles = (R + kTile - 1) / kTile;
+    const int rounds = static_cast<int>((R + kMaxTiles * 256L - 1) / (kMaxTiles * 256L));
+    const dim3 grid(static_cast<unsigned>((R + rounds * 256L - 1) / (rounds * 256L)));
     unsigned *other_key = scratch, *other_order = scratch + R, *count = scratch + 2 * R;
     int passes = 1;
     while (passes < 4 && (v >> (8 * passes)) != 0) ++passes;
     const unsigned *from = nullptr, *from_order = nullptr;
-    const dim3 grid(static_cast<unsigned>(tiles));
     for (int p = 0; p < passes; ++p) {
         const bool last = (passes - p) & 1;  // the passes alternate, the last one ends in key / order
         unsigned *to = last ? key : other_key, *to_order = last ? order : other_order;
         const long* tok = p == 0 ? tokens : nullptr;
-        hipLaunchKernelGGL(digit_count_kernel, grid, dim3(256), 0, s, tok, from, v, padding, count, R, 8 * p);
-        hipLaunchKernelGGL(digit_scan_kernel, dim3(1), dim3(1024), 0, s, count, tiles * kDigits);
-        hipLaunchKernelGGL(digit_scatter_kernel, grid, dim3(256), 0, s, tok, from, from_order, v, padding, count,
-                           to, to_order, R, 8 * p);
+        hipLaunchKernelGGL(digit_count_kernel, grid, dim3(256), 0, s, tok, from, v, padding, count, R, rounds, 8 * p);
+        hipLaunchKernelGGL(digit_move_kernel, grid, dim3(256), 0, s, tok, from, from_order, v, padding, count, to,
+                           to_order, R, rounds, 8 * p);
         from = to;
         from_order = to_order;
     }
     return static_cast<int>(hipGetLastError());
 }
 
-// floats of scratch that nf_embedding_bwd needs
-long nf_embedding_bwd_floats(long R, long C) {
+// 32-bit words of scratch that nf_embedding_bwd needs (`ordered`: with key and order given)
+long nf_embedding_bwd_words(long R, long C, int ordered) {
     const int chunk = chunk_of(R, static_cast<int>((C + 511) / 512));
-    return 2 * ((R + chunk - 1) / chunk) * C;
+    return 2 * ((R + chunk - 1) / chunk) * C + (ordered ? 0 : 2 * R + nf_token_order_words(R));
 }
 
-// key / order: from nf_token_order.  dx: B T rows of C.  dw [V][C]: written everywhere, or
+// key / order: from nf_token_order, or both null: made here from the tokens.  dx: B T rows of C.  dw [V][C]: written everywhere, or
 // (accumulate) added to where tokens are.  dp (may be null): rows 0 .. T - 1 are written.
 // type: of dx; grad_type: of dw and dp (0, or the type of dx).
-int nf_embedding_bwd(const unsigned* key, const unsigned* order, const void* dx, void* dw, void* dp,
-                     float* scratch, int type, int grad_type, long B, long T, long V, long C, float scale,
+int nf_embedding_bwd(const long* tokens, const unsigned* key, const unsigned* order, long padding,
+                     const void* dx, void* dw, void* dp, float* scratch, int type, int grad_type, long B, long T, long V, long C, float scale,
                      int accumulate, unsigned limit, unsigned long long seed, const long* step_at,
                      unsigned step, long first, hipStream_t s) {
     if (B <= 0 || T <= 0 || V <= 0 || C <= 0 || limit > 65535u || first < 0) return -1;
-    if (V >= (1L << 31) || C >= (1L << 24) || B >= (1L << 31) || T >= (1L << 31) || B * T >= (1L << 31)) return -3;
+    if (V >= (1L << 31) || C >= (1L << 25) || B >= (1L << 31) || T >= (1L << 31) || B * T >= (1L << 31)) return -3;
     if (grad_type != 0 && grad_type != type) return -1;
     BwdArgs a = {};
-    a.key = key; a.order = order; a.dx = dx; a.dw = dw; a.dp = dp;
+    a.dx = dx; a.dw = dw; a.dp = dp;
     a.B = B; a.T = T; a.V = V; a.C = C;
     a.R = static_cast<int>(B * T);
     a.slabs = static_cast<int>((C + 511) / 512);
@@ -515,6 +512,15 @@ int nf_embedding_bwd(const unsigned* key, const unsigned* order, const void* dx,
     a.scale = scale;
     a.d = drop_rows(limit, seed, step_at, step, first);
     if (static_cast<long>(a.chunks) * a.slabs > (1L << 22)) return -3;
+    if (key == nullptr || order == nullptr) {
+        unsigned* words = reinterpret_cast<unsigned*>(scratch + 2 * static_cast<long>(a.chunks) * C);
+        const int status = nf_token_order(tokens, words, words + a.R, words + 2L * a.R, a.R, V, padding, s);
+        if (status != 0) return status;
+        key = words;
+        order = words + a.R;
+    }
+    a.key = key;
+    a.order = order;
     switch (type * 4 + grad_type) {
     case 0: return bwd<float, float>(a, s);
     case 4: return bwd<bf16, float>(a, s);

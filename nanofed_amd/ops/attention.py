@@ -16,7 +16,8 @@ layer; this serves the GPT-2 configuration of the benchmark suite.
 
 from __future__ import annotations
 
-from ctypes import Structure, byref, c_float, c_int, c_long, c_uint, c_ulong, c_void_p
+import struct
+from ctypes import c_int, c_long, c_void_p
 
 import torch
 import torch.nn.functional as F
@@ -26,13 +27,14 @@ from nanofed_amd.core.exceptions import DeviceError
 from . import library
 from .dropout import check_key, limit_of, philox_words
 
-P, I = c_void_p, c_int
+P, I, L = c_void_p, c_int, c_long
 _SIGS = {
     "nf_attn_seq_multiple": ([], I),
     "nf_attn_fwd": ([P, P, P, I, I, I, P], I),
     "nf_attn_bwd": ([P, P, P, P, P, P, I, I, I, P], I),
     "nf_attn_set_split": ([I], None),
     "nf_attention_args_size": ([], I),
+    "nf_attention_fwd_floats": ([P], L),
     "nf_attention": ([P, I, I, P], I),
 }
 _fns: dict[str, object] = {}
@@ -130,44 +132,56 @@ def causal_attention_bwd(qkv: torch.Tensor, out: torch.Tensor, lse: torch.Tensor
 MAX_HEAD_DIM = 128
 _TYPES = {torch.bfloat16: 1, torch.float16: 2}
 
-
-class _Strides(Structure):
-    _fields_ = [("b", c_long), ("t", c_long), ("h", c_long)]
-
-
-class _Args(Structure):
-    """Mirror of ``AttnArgs`` in csrc/hip/attention_general.hip."""
-
-    _fields_ = [
-        ("q", P), ("k", P), ("v", P), ("out", P), ("lse", P), ("dout", P), ("dq", P), ("dk", P),
-        ("dv", P), ("delta", P), ("qlen", P), ("klen", P), ("step_at", P),
-        ("s_q", _Strides), ("s_k", _Strides), ("s_v", _Strides), ("s_out", _Strides),
-        ("s_dout", _Strides), ("s_dq", _Strides), ("s_dk", _Strides), ("s_dv", _Strides),
-        ("seed", c_ulong), ("first_head", c_ulong),
-        ("B", I), ("Tq", I), ("Tk", I), ("H", I), ("Hk", I), ("D", I), ("causal", I),
-        ("scale", c_float), ("up", c_float), ("limit", c_uint), ("step", c_uint),
-    ]
+# ``AttnArgs`` of csrc/hip/attention_general.hip: addresses (q k v out lse dout dq dk dv delta, the
+# lengths, the step in memory), distances between sequences, rows and heads (q k v out dout dq dk
+# dv), seed and first head, sizes, scale and factor of what is kept, threshold and step, scratch
+_PACK = struct.Struct("@13P24q2Q7i2f2IPi0q")
+_NONE = (0, 0, 0, 0)
 
 
-def _operand(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, written: bool) -> _Strides:
-    """Checks a ``[B, T, heads, D]`` operand; its distances between sequences, rows and heads."""
-    if t.dtype != like.dtype or t.device != like.device:
+class _Args:
+    """What both directions share, checked."""
+
+    __slots__ = ("B", "Tq", "Tk", "H", "Hk", "D", "causal", "scale", "limit", "up", "seed", "step_at",
+                 "step", "first_head", "q", "k", "v", "qlen", "klen")
+
+    def pack(self, lse: int, out: tuple, dout=_NONE, dq=_NONE, dk=_NONE, dv=_NONE, delta: int = 0,
+             parts: int = 0) -> bytes:
+        q, k, v = self.q, self.k, self.v
+        return _PACK.pack(
+            q[0], k[0], v[0], out[0], lse, dout[0], dq[0], dk[0], dv[0], delta, self.qlen, self.klen,
+            self.step_at, *q[1:], *k[1:], *v[1:], *out[1:], *dout[1:], *dq[1:], *dk[1:], *dv[1:],
+            self.seed, self.first_head, self.B, self.Tq, self.Tk, self.H, self.Hk, self.D, self.causal,
+            self.scale, self.up, self.limit, self.step, parts, 0)
+
+
+def _operand(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, written: bool) -> tuple:
+    """Checks a ``[B, T, heads, D]`` operand; its address and the distances between its sequences,
+    rows and heads."""
+    if t.dtype is not like.dtype or t.device != like.device:
         raise DeviceError(f"attention: {name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise DeviceError(f"attention: {name} must be {list(shape)}, got {list(t.shape)}")
-    strides = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
-    if shape[3] > 1 and strides[3] != 1:
+    at = t.data_ptr()
+    b, s, h, d = t.stride()
+    if d == 1 and not (at & 15 or (b | s | h) & 7) and b and s and h and s < 1 << 24:
+        return at, b, s, h
+    # lengths of one have any distance, and distances of 0 are fine to read
+    strides = [0 if n == 1 else x for n, x in zip(shape, (b, s, h))]
+    if shape[3] > 1 and d != 1:
         raise DeviceError(f"attention: the columns of {name} must be contiguous")
-    if t.device.type == "cuda" and (t.data_ptr() % 16 or any(s % 8 for s in strides[:3])):
+    if t.is_cuda and (at & 15 or any(x & 7 for x in strides)):
         raise DeviceError(f"attention: rows of {name} must start at multiples of 16 bytes")
-    if written and any(n > 1 and s == 0 for n, s in zip(t.shape, strides)):
+    if strides[1] >= 1 << 24:
+        raise DeviceError(f"attention: rows of {name} must be less than 2^24 elements apart")
+    if written and any(n > 1 and x == 0 for n, x in zip(shape, strides)):
         raise DeviceError(f"attention: {name} is written and must not be expanded")
-    return _Strides(*strides[:3])
+    return (at, *strides)
 
 
-def _lengths(t: torch.Tensor | None, name: str, like: torch.Tensor) -> int | None:
+def _lengths(t: torch.Tensor | None, name: str, like: torch.Tensor) -> int:
     if t is None:
-        return None
+        return 0
     if t.dtype != torch.int32 or not t.is_contiguous() or t.shape != like.shape[:1] or t.device != like.device:
         raise DeviceError(f"attention: {name} must be {like.shape[0]} contiguous int32 on {like.device}")
     return t.data_ptr()
@@ -178,52 +192,41 @@ def _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step
         raise DeviceError("attention: q, k and v are [batch, length, heads, head dimension]")
     if q.dtype not in _TYPES and not (q.device.type == "cpu" and q.dtype in (torch.float32, torch.float64)):
         raise DeviceError(f"attention: bfloat16 or float16, got {q.dtype}")
-    B, Tq, H, D = q.shape
-    Tk, Hk = k.shape[1], k.shape[2]
+    a = _Args()
+    shape = q.shape
+    a.B, a.Tq, a.H, a.D = B, Tq, H, D = shape
+    _, a.Tk, a.Hk, _ = k.shape
+    Tk, Hk = a.Tk, a.Hk
     if Hk == 0 or H % Hk:
         raise DeviceError(f"attention: {H} query heads do not share {Hk} key heads evenly")
     if not 0 < D <= MAX_HEAD_DIM or D % 8:
         raise DeviceError(f"attention: the head dimension must be a multiple of 8 up to {MAX_HEAD_DIM}, got {D}")
     if max(Tq, Tk) > 1 << 22 or B * H > 1 << 23:
         raise DeviceError("attention: lengths go up to 2^22, batch * heads up to 2^23")
-    scale = D**-0.5 if scale is None else float(scale)
+    a.scale = scale = D**-0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise DeviceError("attention: the scale must be positive")
-    limit = limit_of(dropout, 8, "attention")
+    a.limit = limit_of(dropout, 8, "attention")
+    a.up = 256 / (256 - a.limit)
     check_key(seed, step, q.device, "attention")
-    if first_batch < 0:
-        raise DeviceError("attention: first_batch must not be negative")
-    a = _Args(B=B, Tq=Tq, Tk=Tk, H=H, Hk=Hk, D=D, causal=bool(causal), scale=scale, limit=limit,
-              up=256 / (256 - limit), seed=seed, first_head=first_batch * H)
-    for name, t, shape in (("q", q, (B, Tq, H, D)), ("k", k, (B, Tk, Hk, D)), ("v", v, (B, Tk, Hk, D))):
-        setattr(a, "s_" + name, _operand(t, name, shape, q, False))
-        setattr(a, name, t.data_ptr())
+    a.seed = seed
+    a.step_at, a.step = (step.data_ptr(), 0) if isinstance(step, torch.Tensor) else (0, step)
+    if not 0 <= first_batch < 1 << 32:
+        raise DeviceError("attention: first_batch must not be negative (nor pass 2^32)")
+    a.first_head = first_batch * H
+    a.causal = bool(causal)
+    shared = (B, Tk, Hk, D)
+    a.q = _operand(q, "q", shape, q, False)
+    a.k = _operand(k, "k", shared, q, False)
+    a.v = _operand(v, "v", shared, q, False)
     a.qlen, a.klen = _lengths(q_lengths, "q_lengths", q), _lengths(k_lengths, "k_lengths", q)
-    if isinstance(step, torch.Tensor):
-        a.step_at = step.data_ptr()
-    else:
-        a.step = step
     return a
-
-
-def _add(a: _Args, q: torch.Tensor, **operands: torch.Tensor) -> None:
-    for name, t in operands.items():
-        heads, T = (a.Hk, a.Tk) if name in ("dk", "dv") else (a.H, a.Tq)
-        setattr(a, "s_" + name, _operand(t, name, (a.B, T, heads, a.D), q, name != "dout"))
-        setattr(a, name, t.data_ptr())
 
 
 def _check_lse(lse: torch.Tensor, a: _Args, q: torch.Tensor) -> None:
     if (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device
-            or tuple(lse.shape) != (a.B, a.H, a.Tq)):
+            or lse.shape != (a.B, a.H, a.Tq)):
         raise DeviceError(f"attention: lse must be contiguous float32 [{a.B}, {a.H}, {a.Tq}] on {q.device}")
-
-
-def _launch(a: _Args, q: torch.Tensor, backward: bool) -> None:
-    with library.on_device(q.device):
-        library.check(_fn("nf_attention")(byref(a), _TYPES[q.dtype], int(backward),
-                                          library.stream_ptr(q.device)),
-                      "attention_bwd" if backward else "attention_fwd")
 
 
 def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor | None = None,
@@ -256,22 +259,29 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if lse is None:
         lse = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
-    _add(a, q, out=out)
+    to = _operand(out, "out", q.shape, q, True)
     _check_lse(lse, a, q)
-    if q.numel() == 0:
+    if a.B == 0 or a.Tq == 0:
         return out, lse
     if a.Tk == 0:
         out.zero_()
         lse.fill_(float("-inf"))
         return out, lse
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         prob, kept, sums = _probabilities(a, q, k, q_lengths, k_lengths, step)
         lse.copy_(sums)
         y = (prob * kept) @ _shared(a, v, k_lengths)
         out.copy_(y.transpose(1, 2))
         return out, lse
-    a.lse = lse.data_ptr()
-    _launch(a, q, False)
+    packed, dev = a.pack(lse.data_ptr(), to), q.device
+    with library.on_device(dev):
+        floats = _fn("nf_attention_fwd_floats")(packed)
+        if floats:
+            # (scratch of its own for every call: the allocator hands it on in stream order, and a
+            # captured call's belongs to its graph)
+            parts = torch.empty(floats, dtype=torch.float32, device=dev)
+            packed = a.pack(lse.data_ptr(), to, parts=parts.data_ptr())
+        library.check(_fn("nf_attention")(packed, _TYPES[q.dtype], 0, library.stream_ptr(dev)), "attention_fwd")
     return out, lse
 
 
@@ -287,13 +297,16 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     that share it in a fixed order, without atomics.  ``dq``, ``dk``, ``dv`` must not overlap what is
     read."""
     a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
-    _add(a, q, out=out, dout=dout, dq=dq, dk=dk, dv=dv)
+    shape, shared = q.shape, k.shape
+    operands = (_operand(out, "out", shape, q, False), _operand(dout, "dout", shape, q, False),
+                _operand(dq, "dq", shape, q, True), _operand(dk, "dk", shared, q, True),
+                _operand(dv, "dv", shared, q, True))
     _check_lse(lse, a, q)
-    if q.numel() == 0 or a.Tk == 0:
+    if a.B == 0 or a.Tq == 0 or a.Tk == 0:
         for t in (dq, dk, dv):
             t.zero_()
         return
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         prob, kept, _ = _probabilities(a, q, k, q_lengths, k_lengths, step)
         rows = _valid(a, q_lengths, a.Tq).view(a.B, 1, a.Tq, 1)
         qf = _masked(q, rows)
@@ -305,9 +318,11 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
         for t, g in ((dk, ds.transpose(-1, -2) @ qf), (dv, gv)):
             t.copy_(g.view(a.B, a.Hk, a.H // a.Hk, a.Tk, a.D).sum(2).transpose(1, 2))
         return
-    delta = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
-    a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
-    _launch(a, q, True)
+    dev = q.device
+    delta = torch.empty(a.B * a.H * a.Tq, dtype=torch.float32, device=dev)
+    with library.on_device(dev):
+        library.check(_fn("nf_attention")(a.pack(lse.data_ptr(), *operands, delta=delta.data_ptr()),
+                                          _TYPES[q.dtype], 1, library.stream_ptr(dev)), "attention_bwd")
 
 
 def _valid(a: _Args, lengths: torch.Tensor | None, T: int) -> torch.Tensor:

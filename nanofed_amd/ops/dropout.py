@@ -63,11 +63,11 @@ def check_key(seed: int, step: "int | torch.Tensor", device: torch.device, what:
         raise DeviceError(f"{what}: the step must be a 32-bit unsigned number")
 
 
-def step_args(step: "int | torch.Tensor") -> tuple[c_void_p, int]:
+def step_args(step: "int | torch.Tensor") -> tuple[int | None, int]:
     """(address of the step in device memory, its value when it is a plain number)."""
     if isinstance(step, torch.Tensor):
-        return c_void_p(step.data_ptr()), 0
-    return c_void_p(0), step
+        return step.data_ptr(), 0
+    return None, step
 
 
 def philox_words(seed: int, step: "int | torch.Tensor", c0: torch.Tensor, c1: torch.Tensor,
@@ -96,16 +96,6 @@ def kept_rows(n: int, limit: int, seed: int, step: "int | torch.Tensor", first: 
 
 
 # -- the operator -------------------------------------------------------------------------
-def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
-    """(rows, columns, distance) of a tensor that is rows of contiguous columns: contiguous
-    tensors are one row."""
-    if t.is_contiguous():
-        return 1, t.numel(), t.numel()
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
-        return t.shape[0], t.shape[1], t.stride(0)
-    raise DeviceError(f"{name} must be contiguous, or rows of contiguous columns")
-
-
 def dropout_fwd(x: torch.Tensor, p: float, *, seed: int, step: "int | torch.Tensor" = 0,
                 residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
                 first: int = 0) -> torch.Tensor:
@@ -137,19 +127,19 @@ def dropout_fwd(x: torch.Tensor, p: float, *, seed: int, step: "int | torch.Tens
         return out
     if x.numel() == 0:
         return out
-    parts = [_rows(t, n) for t, n in ((x, "x"), (out, "out"), (residual, "residual")) if t is not None]
-    if any(r > 1 for r, _, _ in parts):  # some tensor has rows apart: all are walked by rows
-        R, C = x.shape
-        ld = [C if r == 1 else d for r, _, d in parts]
-    else:
-        R, C = 1, x.numel()
-        ld = [C] * len(parts)
+    R, C, ld, ldr, ldo = 1, x.numel(), 0, 0, 0
+    if not (x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous())):
+        # some tensor has rows apart: all are walked by rows
+        for t, name in ((x, "x"), (out, "out"), (residual, "residual")):
+            if t is not None and (t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]):
+                raise DeviceError(f"dropout: {name} must be contiguous, or rows of contiguous columns")
+        (R, C), ld, ldo = x.shape, x.stride(0), out.stride(0)
+        ldr = residual.stride(0) if residual is not None else 0
     at, number = step_args(step)
     with library.on_device(x.device):
         library.check(_fn("nf_dropout")(
             x.data_ptr(), residual.data_ptr() if residual is not None else None, out.data_ptr(),
-            FLOAT_TYPES[x.dtype], R, C, ld[0], ld[2] if residual is not None else 0, ld[1], limit,
-            seed, at, number, first, library.stream_ptr(x.device)), "dropout")
+            FLOAT_TYPES[x.dtype], R, C, ld, ldr, ldo, limit, seed, at, number, first, library.stream_ptr(x.device)), "dropout")
     return out
 
 

@@ -29,8 +29,8 @@ _SIGS = {
     "nf_embedding_fwd": ([P, P, P, P, I, L, L, L, L, FL, U, UL, P, U, L, P], I),
     "nf_token_order_words": ([L], L),
     "nf_token_order": ([P, P, P, P, L, L, L, P], I),
-    "nf_embedding_bwd_floats": ([L, L], L),
-    "nf_embedding_bwd": ([P, P, P, P, P, P, I, I, L, L, L, L, FL, I, U, UL, P, U, L, P], I),
+    "nf_embedding_bwd_words": ([L, L, I], L),
+    "nf_embedding_bwd": ([P, P, P, L, P, P, P, P, I, I, L, L, L, L, FL, I, U, UL, P, U, L, P], I),
 }
 _fns: dict[str, object] = {}
 
@@ -48,11 +48,15 @@ def symbols() -> list[str]:
     return sorted(_SIGS)
 
 
+def _address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def _need(t: torch.Tensor, shape: tuple, dtypes, device: torch.device, name: str) -> None:
     if t.dtype not in dtypes or t.device != device or not t.is_contiguous():
         raise DeviceError(f"embedding: {name} must be contiguous {' or '.join(map(str, dtypes))} on "
                           f"{device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise DeviceError(f"embedding: {name} must be {list(shape)}, got {list(t.shape)}")
 
 
@@ -104,8 +108,7 @@ def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor |
     at, number = step_args(step)
     with library.on_device(dev):
         library.check(_fn("nf_embedding_fwd")(
-            tokens.data_ptr(), table.data_ptr(), positions.data_ptr() if positions is not None else None,
-            out.data_ptr(), FLOAT_TYPES[table.dtype], B * T, T, V, C, scale, limit, seed, at, number,
+            tokens.data_ptr(), table.data_ptr(), _address(positions), out.data_ptr(), FLOAT_TYPES[table.dtype], B * T, T, V, C, scale, limit, seed, at, number,
             first, library.stream_ptr(dev)), "embedding_fwd")
     return out
 
@@ -202,14 +205,14 @@ def embedding_bwd(tokens: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor
         else:
             dtable.copy_(acc)
         return
-    key, rows = order if order is not None else token_order(tokens, V, padding_idx)
+    key, rows = order if order is not None else (None, None)
     at, number = step_args(step)
     # (scratch of its own for every call: the allocator hands it on in stream order, and a captured
     # call's belongs to its graph)
-    scratch = torch.empty(_fn("nf_embedding_bwd_floats")(R, C), dtype=torch.float32, device=dev)
+    scratch = torch.empty(_fn("nf_embedding_bwd_words")(R, C, order is not None), dtype=torch.float32, device=dev)
     with library.on_device(dev):
         library.check(_fn("nf_embedding_bwd")(
-            key.data_ptr(), rows.data_ptr(), dout.data_ptr(), dtable.data_ptr(),
-            dpositions.data_ptr() if dpositions is not None else None, scratch.data_ptr(),
-            FLOAT_TYPES[dout.dtype], FLOAT_TYPES[dtable.dtype], B, T, V, C, scale, int(accumulate), limit, seed, at, number,
-            first, library.stream_ptr(dev)), "embedding_bwd")
+            tokens.data_ptr(), _address(key), _address(rows), padding, dout.data_ptr(), dtable.data_ptr(),
+            _address(dpositions), scratch.data_ptr(), FLOAT_TYPES[dout.dtype], FLOAT_TYPES[dtable.dtype],
+            B, T, V, C, scale, accumulate, limit, seed, at, number, first, library.stream_ptr(dev)),
+            "embedding_bwd")

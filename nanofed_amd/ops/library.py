@@ -86,8 +86,14 @@ def declare(name: str, argtypes: list, restype=c_int):
     return fn
 
 
+# the stream's handle without making a Stream object (a third of a small launch's host time)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device | None = None) -> c_void_p:
     """The current HIP stream of ``device`` as a ``hipStream_t``."""
+    if _raw_stream is not None and device is not None and device.index is not None:
+        return c_void_p(_raw_stream(device.index))
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 

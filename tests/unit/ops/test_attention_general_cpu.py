@@ -1,7 +1,6 @@
 """The PyTorch paths of ``attention_fwd`` / ``attention_bwd`` against the definition in 64 bits
 and against differences, and what the operator refuses."""
 
-import ctypes
 import math
 
 import pytest
@@ -148,7 +147,7 @@ def test_refusals():
 
 
 def test_argument_block_mirrors_the_kernels():
-    assert ctypes.sizeof(A._Args) == library.hip_lib().nf_attention_args_size()
+    assert A._PACK.size == library.hip_lib().nf_attention_args_size()
 
 
 def test_launcher_refuses_what_the_kernels_cannot_take():
@@ -156,16 +155,20 @@ def test_launcher_refuses_what_the_kernels_cannot_take():
     launch."""
     fn = A._fn("nf_attention")
 
-    def code(type_=1, backward=0, **over):
-        a = A._Args(q=4096, k=4096, v=4096, out=4096, lse=4096, dout=4096, dq=4096, dk=4096, dv=4096, delta=4096,
-                    B=1, Tq=1, Tk=1, H=2, Hk=1, D=64, scale=1.0, up=1.0)
-        for name, value in over.items():
-            setattr(a, name, value)
-        return fn(ctypes.byref(a), type_, backward, None)
+    def code(type_=1, backward=0, B=1, Tq=1, Tk=1, H=2, Hk=1, D=64, scale=1.0, limit=0, v=(4096, 8, 8, 8),
+             q=4096, lse=4096, dv=4096, delta=4096):
+        a = A._Args()
+        a.B, a.Tq, a.Tk, a.H, a.Hk, a.D, a.scale, a.limit, a.up = B, Tq, Tk, H, Hk, D, scale, limit, 1.0
+        a.causal = a.seed = a.step_at = a.step = a.first_head = a.qlen = a.klen = 0
+        some = (4096, 8, 8, 8)
+        a.q, a.k, a.v = (q, 8, 8, 8), some, v
+        return fn(a.pack(lse, some, some, some, some, (dv, 8, 8, 8), delta), type_, backward, None)
 
     assert code(B=0) == -1 and code(Tk=0) == -1 and code(Hk=0) == -1 and code(H=3, Hk=2) == -1
     assert code(D=12) == -1 and code(D=136) == -1 and code(limit=256) == -1 and code(scale=0.0) == -1
     assert code(scale=math.nan) == -1 and code(type_=0) == -1
     assert code(Tq=(1 << 22) + 1) == -3 and code(B=1 << 23) == -3
-    assert code(q=4104) == -2 and code(lse=None) == -2 and code(s_v=A._Strides(0, 4, 0)) == -2
-    assert code(backward=1, delta=None) == -2 and code(backward=1, dv=None) == -2
+    assert code(q=4104) == -2 and code(lse=0) == -2 and code(v=(4096, 0, 4, 0)) == -2
+    assert code(v=(4096, 0, 1 << 24, 0)) == -2
+    assert code(backward=1, delta=0) == -2 and code(backward=1, dv=0) == -2
+    assert code(Tk=4096) == -2  # many keys for one query, and no scratch for the parts

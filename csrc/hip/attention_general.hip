@@ -29,6 +29,7 @@
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "../common/philox.h"
 #include "nf_device.h"
@@ -82,8 +83,8 @@ struct AttnArgs {
     int B, Tq, Tk, H, Hk, D, causal;
     float scale, up;
     unsigned limit, step;
-    float* parts;             // few queries: partial results of the key chunks, or null (one chunk)
-    int chunk;                // keys per chunk
+    float* parts;             // few queries: partial results of the key chunks
+    int target;               // few queries: workgroups to cut the keys for (0: not cut)
 };
 
 // -- tiles ------------------------------------------------------------------------------------
@@ -407,46 +408,94 @@ attn_fwd_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Forward of few queries (queries x heads per key head <= 32) against many keys: the queries of
 // all heads that share a key head are the columns of one tile, so the keys are read once for all
-// of them.  Bound by reading the keys and values.  A workgroup takes a chunk of the keys (grid =
-// sequence and key head, chunk), its waves every fourth 32 of them; a wave reads K straight into
-// operand fragments and V through LDS of its own (no barrier in the loop), one tile ahead.  The
-// waves are joined through LDS, the chunks by attn_join_kernel.
-constexpr int kFew = 32;
+// of them.  Bound by reading the keys and values.  A workgroup takes a chunk of the keys, its
+// waves every fourth 32 of them, through LDS of their own (no barrier in the loop), one tile ahead
+// in registers.  The waves are joined through LDS, the chunks by attn_join_kernel.
+//
+// The chunks are cut on the device, from the lengths: about `target` of equal size over all
+// sequences, so a batch of short and long ones still fills the chip evenly.  What a chunk costs
+// apart from its keys (the first load, the joins) is worth some hundred keys, so there are no more
+// of them than workgroups run at once.  (Chunks of 256 / 1024 keys for every sequence measured
+// 28.7 / 23.8 us on four caches of up to 8191 keys x 8 heads x 128, equal shares of the 84 MB KTIME.)
+constexpr int kFew = 32, kFewMaxBatch = 512;
 
-// parts: [B Hk][chunks][rows][DP] of O, then [B Hk][chunks][rows] x (m, l)
+struct Chunk { int b, hk, count, at, size; Seq seq; };  // chunk `at` of `count` of (b, hk), keys per chunk
+
+__device__ __forceinline__ int few_keys(const Seq& s) { return s.m > 0 ? s.n : 0; }
+
+__device__ __forceinline__ int lane_sum(int v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+
+// Keys per chunk, given the number of keys of all sequences (B * Hk < target, so the sum of what
+// the sequences' last chunks are short of adds less than `target` workgroups).
+__device__ __forceinline__ int few_size(const AttnArgs& a, long keys) {
+    return static_cast<int>(max(128L, ((keys * a.Hk + a.target - 1) / a.target + 127) & ~127L));
+}
+
+// Which chunk workgroup `id` has; b < 0: none.  All lanes; lane i looks at sequences i, i + 64, ...
+__device__ __forceinline__ Chunk few_chunk(const AttnArgs& a, int id, int lane) {
+    if (a.target == 0) return {id / a.Hk, id % a.Hk, 1, 0, a.Tk, sequence(a, id / a.Hk)};
+    const Seq mine0 = lane < a.B ? sequence(a, lane) : Seq{0, 0, 0};
+    long keys = few_keys(mine0);
+    for (int i = lane + 64; i < a.B; i += 64) keys += few_keys(sequence(a, i));
+    const int size = few_size(a, lane_sum(static_cast<int>(keys)));
+    int before = 0;  // parts of the sequences before
+    for (int i0 = 0; i0 < a.B; i0 += 64) {
+        const Seq mine = i0 == 0 ? mine0 : (i0 + lane < a.B ? sequence(a, i0 + lane) : Seq{0, 0, 0});
+        const int count = (few_keys(mine) + size - 1) / size;
+        int x = count;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(x, off, 64);
+            if (lane >= off) x += y;
+        }
+        const unsigned long here = __ballot(id < (before + x) * a.Hk);
+        if (here != 0) {
+            const int who = __builtin_ctzl(here), c = __builtin_amdgcn_readlane(count, who);
+            const int at = id - (before + __builtin_amdgcn_readlane(x, who) - c) * a.Hk, k = at / a.Hk;
+            const Seq s = {__builtin_amdgcn_readlane(mine.m, who), __builtin_amdgcn_readlane(mine.n, who),
+                           __builtin_amdgcn_readlane(mine.off, who)};
+            return {i0 + who, at - k * a.Hk, c, k, size, s};
+        }
+        before += __builtin_amdgcn_readlane(x, 63);
+    }
+    return {-1, 0, 0, 0, 0, {0, 0, 0}};
+}
+
 template <class E, int DP>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 attn_few_kernel(AttnArgs a) {
     typedef Tile<E, DP, 32> T;
     typedef typename T::x8 x8;
-    constexpr int NB = DP / 32, KS = DP / 16, kVPer = 32 * T::kPieces / 64;
+    constexpr int NB = DP / 32, KS = DP / 16, kPer = 32 * T::kPieces / 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int bh = blockIdx.x, b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
     const int lane = threadIdx.x & 63, n = lane & 31, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Seq sq = sequence(a, b);
+    const Chunk me = few_chunk(a, blockIdx.x, lane);
+    if (me.b < 0) return;
+    const int b = me.b, hk = me.hk, group = a.H / a.Hk;
+    const Seq sq = me.seq;
     const int rows = a.Tq * group, qi = n / group, h = hk * group + n % group;
     const bool in = n < rows && qi < sq.m;
     const int seen = (in ? keys_seen(sq, qi) : 0) - 4 * hh;
-    const int k0 = blockIdx.y * a.chunk, k1 = min(sq.m > 0 ? sq.n : 0, k0 + a.chunk);
-    char* lds = smem + wave * T::kBytes;
+    const int k0 = me.at * me.size, k1 = min(sq.m > 0 ? sq.n : 0, k0 + me.size);
+    char* lds = smem + wave * 2 * T::kBytes;  // K, V
     const typename T::Lane at = T::lane_offsets(lane);
     x8 qf[KS];
     own_row<E, DP>(static_cast<const E*>(a.q) + b * a.sq.b + qi * a.sq.t + h * a.sq.h, in, a.D, hh, qf);
-    unsigned koff[KS], voff[kVPer];
+    unsigned koff[kPer], voff[kPer];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const int c = ks * 16 + 8 * hh;
-        koff[ks] = c < a.D ? static_cast<unsigned>(n * a.sk.t + c) * 2u : 0x80000000u;
-    }
-#pragma unroll
-    for (int i = 0; i < kVPer; ++i) {
-        const int idx = lane + 64 * i, c = (idx % T::kPieces) * 8;
-        voff[i] = c < a.D ? static_cast<unsigned>((idx / T::kPieces) * a.sv.t + c) * 2u : 0x80000000u;
+    for (int i = 0; i < kPer; ++i) {
+        const int idx = lane + 64 * i, r = idx / T::kPieces, c = (idx % T::kPieces) * 8;
+        koff[i] = c < a.D ? static_cast<unsigned>(r * a.sk.t + c) * 2u : 0x80000000u;
+        voff[i] = c < a.D ? static_cast<unsigned>(r * a.sv.t + c) * 2u : 0x80000000u;
     }
     const E* kb = static_cast<const E*>(a.k) + b * a.sk.b + hk * a.sk.h;
     const E* vb = static_cast<const E*>(a.v) + b * a.sv.b + hk * a.sv.h;
-    u32x4 kr[KS], vr[kVPer];
+    u32x4 kr[kPer], vr[kPer];
     auto fetch = [&](int key0) {  // rows behind the last key read as 0
         const long last = min(sq.n - key0, 32) - 1;
         const __amdgpu_buffer_rsrc_t kd = __builtin_amdgcn_make_buffer_rsrc(
@@ -454,10 +503,10 @@ attn_few_kernel(AttnArgs a) {
         const __amdgpu_buffer_rsrc_t vd = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<E*>(vb + key0 * a.sv.t), 0, static_cast<int>((last * a.sv.t + a.D) * 2), 0x00020000);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-            kr[ks] = __builtin_amdgcn_raw_buffer_load_b128(kd, static_cast<int>(koff[ks]), 0, 0);
+        for (int i = 0; i < kPer; ++i)
+            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(kd, static_cast<int>(koff[i]), 0, 0);
 #pragma unroll
-        for (int i = 0; i < kVPer; ++i)
+        for (int i = 0; i < kPer; ++i)
             vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vd, static_cast<int>(voff[i]), 0, 0);
     };
     f32x16 o[NB];
@@ -468,18 +517,19 @@ attn_few_kernel(AttnArgs a) {
     int key0 = k0 + wave * 32;
     if (key0 < k1) fetch(key0);
     for (; key0 < k1; key0 += 128) {
-        f32x16 s = {0};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = mma(__builtin_bit_cast(x8, kr[ks]), qf[ks], s);
         // (the LDS operations of a wave complete in order: the reads of the tile before come first)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int i = 0; i < kVPer; ++i) {
-            const int idx = lane + 64 * i;
-            *reinterpret_cast<u32x4*>(lds + nfix::attn_off(DP, idx / T::kPieces, idx % T::kPieces)) = vr[i];
+        for (int i = 0; i < kPer; ++i) {
+            const int idx = lane + 64 * i, to = nfix::attn_off(DP, idx / T::kPieces, idx % T::kPieces);
+            *reinterpret_cast<u32x4*>(lds + to) = kr[i];
+            *reinterpret_cast<u32x4*>(lds + T::kBytes + to) = vr[i];
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (key0 + 128 < k1) fetch(key0 + 128);
+        f32x16 s = {0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = mma(T::row(lds, at, 0, ks), qf[ks], s);
         const int lim = min(seen, k1 - 4 * hh) - key0;
         float mx = -INFINITY;
 #pragma unroll
@@ -510,8 +560,8 @@ attn_few_kernel(AttnArgs a) {
         const x8 p0 = pack8<E>(s, 0), p1 = pack8<E>(s, 8);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            o[i] = mma(T::tr(lds, at, 0, i), p0, o[i]);
-            o[i] = mma(T::tr(lds, at, 16, i), p1, o[i]);
+            o[i] = mma(T::tr(lds + T::kBytes, at, 0, i), p0, o[i]);
+            o[i] = mma(T::tr(lds + T::kBytes, at, 16, i), p1, o[i]);
         }
     }
     l = sum_halves(l);
@@ -544,10 +594,8 @@ attn_few_kernel(AttnArgs a) {
         }
     }
     if (wave != 0 || n >= rows) return;
-    if (a.parts != nullptr) {
-        const long part = (static_cast<long>(bh) * gridDim.y + blockIdx.y) * rows + n;
-        const long parts = static_cast<long>(gridDim.x) * gridDim.y * rows;
-        if (k0 >= k1) return;  // (a chunk without keys is not read)
+    if (me.count > 1) {
+        const long part = static_cast<long>(blockIdx.x) * rows + n, parts = static_cast<long>(gridDim.x) * rows;
         if (hh == 0) {
             a.parts[parts * DP + 2 * part] = m;
             a.parts[parts * DP + 2 * part + 1] = l;
@@ -582,22 +630,28 @@ attn_few_kernel(AttnArgs a) {
             some ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
 }
 
-// One wave per row: the chunks' maxima and sums, 64 at a time, then their O in order.
+// One wave per row of a sequence that was cut: the chunks' maxima and sums, 64 at a time, then
+// their O in order.
 template <class E, int DP>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int chunks) {
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgroups) {
     const int lane = threadIdx.x & 63, group = a.H / a.Hk, rows = a.Tq * group;
-    const long row = static_cast<long>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long parts = static_cast<long>(a.B) * a.Hk * chunks * rows;
-    if (row >= static_cast<long>(a.B) * a.Hk * rows) return;
-    const long bh = row / rows;
-    const int r = static_cast<int>(row % rows), b = static_cast<int>(bh / a.Hk), hk = static_cast<int>(bh % a.Hk);
+    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (row >= a.B * a.Hk * rows) return;
+    const int bh = row / rows, r = row % rows, b = bh / a.Hk, hk = bh % a.Hk;
     const int qi = r / group, h = hk * group + r % group;
     const Seq sq = sequence(a, b);
-    const int live = qi < sq.m ? (sq.n + a.chunk - 1) / a.chunk : 0;
+    int keys = 0, first = 0;  // keys of all sequences; parts of those before b
+    for (int i = lane; i < a.B; i += 64) keys += few_keys(sequence(a, i));
+    const int size = few_size(a, lane_sum(keys)), count = (few_keys(sq) + size - 1) / size;
+    if (count == 1) return;  // written already
+    for (int i = lane; i < b; i += 64) first += (few_keys(sequence(a, i)) + size - 1) / size;
+    first = lane_sum(first) * a.Hk + hk;  // the parts of chunk c: first + c Hk
+    const int live = qi < sq.m ? count : 0;
+    const long parts = static_cast<long>(workgroups) * rows;
     const float sc2 = a.scale * kLog2e;
     const float* ml = a.parts + parts * DP;
     float m = -INFINITY;
-    for (int c = lane; c < live; c += 64) m = fmaxf(m, ml[2 * ((bh * chunks + c) * rows + r)]);
+    for (int c = lane; c < live; c += 64) m = fmaxf(m, ml[2 * (static_cast<long>(first + c * a.Hk) * rows + r)]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     const float ref = m == -INFINITY ? 0.f : m;
@@ -605,17 +659,17 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int chunks) 
     for (int c0 = 0; c0 < live; c0 += 64) {
         float w = 0.f;
         if (c0 + lane < live) {
-            const long p = (bh * chunks + c0 + lane) * rows + r;
+            const long p = static_cast<long>(first + (c0 + lane) * a.Hk) * rows + r;
             w = exp2_fast((ml[2 * p] - ref) * sc2);
             l = fmaf(ml[2 * p + 1], w, l);
         }
         const int more = min(64, live - c0);
-        const float* o = a.parts + ((bh * chunks + c0) * rows + r) * static_cast<long>(DP);
+        const float* o = a.parts + (static_cast<long>(first + c0 * a.Hk) * rows + r) * DP;
         for (int c1 = 0; c1 < more; c1 += 8) {  // eight parts in flight
             float v0[8], v1[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float* oc = o + min(c1 + u, more - 1) * static_cast<long>(rows) * DP;
+                const float* oc = o + min(c1 + u, more - 1) * static_cast<long>(a.Hk * rows) * DP;
                 v0[u] = oc[lane];
                 if (DP > 64) v1[u] = oc[64 + lane];
             }
@@ -938,30 +992,29 @@ int launch_fwd(const AttnArgs& a, hipStream_t s) {
     return static_cast<int>(hipGetLastError());
 }
 
-// Keys per chunk of attn_few_kernel: about 1024 workgroups where the keys suffice, 128 keys (one
-// tile per wave) at least.  0: not the few-query form.
-int few_chunk(const AttnArgs& a) {
-    if (a.limit != 0 || static_cast<long>(a.Tq) * (a.H / a.Hk) > kFew) return 0;
-    const long per = (static_cast<long>(a.Tk) * a.B * a.Hk + 1023) / 1024;
-    const long chunk = per < 128 ? 128 : (per + 127) / 128 * 128;
-    return static_cast<int>(chunk < a.Tk ? chunk : (a.Tk + 127) / 128 * 128);
+// Workgroups that attn_few_kernel cuts the keys for (0: one per sequence and key head; -1: not the
+// few-query form).
+#ifndef FEWWG
+#define FEWWG 512
+#endif
+constexpr int kFewTarget = FEWWG;
+
+int few_target(const AttnArgs& a) {
+    if (a.limit != 0 || static_cast<long>(a.Tq) * (a.H / a.Hk) > kFew) return -1;
+    return a.B <= kFewMaxBatch && a.B * a.Hk < kFewTarget && a.Tk > 128 ? kFewTarget : 0;
 }
-int few_chunks(const AttnArgs& a, int chunk) { return (a.Tk + chunk - 1) / chunk; }
+int few_workgroups(const AttnArgs& a) { return a.target + a.B * a.Hk; }  // at most
 int padded_dim(int D) { return D <= 64 ? 64 : 128; }
 
 template <class E, int DP>
-int launch_few(AttnArgs a, hipStream_t s) {
-    constexpr int park = 2 * 64 * (DP / 32 * 16 + 2) * 4, v = 4 * Tile<E, DP, 32>::kBytes, lds = park > v ? park : v;
-    const int chunks = few_chunks(a, a.chunk);
-    if (chunks > 1 && a.parts == nullptr) return -2;
-    if (chunks == 1) a.parts = nullptr;
+int launch_few(const AttnArgs& a, hipStream_t s) {
+    constexpr int park = 2 * 64 * (DP / 32 * 16 + 2) * 4, kv = 8 * Tile<E, DP, 32>::kBytes, lds = park > kv ? park : kv;
+    if (a.target != 0 && a.parts == nullptr) return -2;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_few_kernel<E, DP>), lds)) return st;
-    hipLaunchKernelGGL((attn_few_kernel<E, DP>), dim3(a.B * a.Hk, chunks), dim3(256), lds, s, a);
-    if (chunks > 1) {
-        const long rows = static_cast<long>(a.B) * a.H * a.Tq;
-        hipLaunchKernelGGL((attn_join_kernel<E, DP>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, s, a,
-                           chunks);
-    }
+    hipLaunchKernelGGL((attn_few_kernel<E, DP>), dim3(few_workgroups(a)), dim3(256), lds, s, a);
+    if (a.target != 0)
+        hipLaunchKernelGGL((attn_join_kernel<E, DP>), dim3((a.B * a.H * a.Tq + 3) / 4), dim3(256), 0, s, a,
+                           few_workgroups(a));
     return static_cast<int>(hipGetLastError());
 }
 
@@ -979,7 +1032,7 @@ int launch_bwd(const AttnArgs& a, hipStream_t s) {
 template <class E, int DP>
 int launch(const AttnArgs& a, int backward, hipStream_t s) {
     if (backward) return a.limit ? launch_bwd<E, DP, true>(a, s) : launch_bwd<E, DP, false>(a, s);
-    if (a.chunk != 0) return launch_few<E, DP>(a, s);
+    if (a.target >= 0) return launch_few<E, DP>(a, s);
     return a.limit ? launch_fwd<E, DP, true>(a, s) : launch_fwd<E, DP, false>(a, s);
 }
 
@@ -996,11 +1049,9 @@ int nf_attention_args_size() { return static_cast<int>(sizeof(AttnArgs)); }
 
 // floats of scratch that a forward call needs (args->parts)
 long nf_attention_fwd_floats(const AttnArgs* args) {
-    const AttnArgs& a = *args;
-    if (a.Hk <= 0 || a.Tk <= 0) return 0;
-    const int chunk = few_chunk(a);
-    if (chunk == 0 || few_chunks(a, chunk) == 1) return 0;
-    return static_cast<long>(a.B) * a.H * a.Tq * few_chunks(a, chunk) * (2 + padded_dim(a.D));
+    AttnArgs a = *args;
+    if (a.Hk <= 0 || (a.target = few_target(a)) <= 0) return 0;
+    return static_cast<long>(few_workgroups(a)) * a.Tq * (a.H / a.Hk) * (2 + padded_dim(a.D));
 }
 
 // type: 1 bf16, 2 half.  backward 0: reads q, k, v and writes out, lse; 1: reads q, k, v, out,
@@ -1015,8 +1066,7 @@ int nf_attention(const AttnArgs* args, int type, int backward, hipStream_t s) {
     if (backward && (!fits(a.dout, a.sdo) || !fits(a.dq, a.sdq) || !fits(a.dk, a.sdk) ||
                      !fits(a.dv, a.sdv) || a.delta == nullptr))
         return -2;
-    a.chunk = backward ? 0 : few_chunk(a);
-    if (a.chunk != 0 && few_chunks(a, a.chunk) > 65535) return -3;
+    a.target = backward ? -1 : few_target(a);
     if (type == 1) return a.D <= 64 ? launch<bf16, 64>(a, backward, s) : launch<bf16, 128>(a, backward, s);
     if (type == 2) return a.D <= 64 ? launch<half, 64>(a, backward, s) : launch<half, 128>(a, backward, s);
     return -1;

@@ -323,10 +323,9 @@ __device__ __forceinline__ void zero_absent(const BwdArgs& a, long block) {
     G* rows = static_cast<G*>(a.dw) + block * 64 * a.C;
     for (unsigned e = threadIdx.x * 8; e < n; e += 2048) {
         const unsigned r = e / C, end = min(e + 8, n);
-        const unsigned long bits = absent >> r;
-        if (end == e + 8 && (bits & 1) && ((r + 1) * C >= end || ((bits & 2) && (r + 2) * C >= end))) {
-            store8(rows + e, zero);
-        } else {
+        if (end <= (r + 1) * C) {
+            if ((absent >> r) & 1) store_unit(rows + e, static_cast<int>(end - e), zero);
+        } else {  // the unit spans rows
             for (unsigned i = e; i < end; ++i)
                 if ((absent >> (i / C)) & 1) rows[i] = static_cast<G>(0.f);
         }

@@ -244,6 +244,11 @@ __device__ __forceinline__ bool kept(const unsigned (&w)[4], int r, unsigned lim
 // of the others would be turned into selects that all tiles pay for.
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
+// Keeps a group of LDS reads together and ahead of what follows.  Left alone the compiler puts every
+// read right before the MFMA that takes it, into the same registers, and each product then waits
+// for an LDS round trip.
+__device__ __forceinline__ void reads_first() { __builtin_amdgcn_sched_barrier(0); }
+
 // row of accumulator register r without the lane's part (4 (lane >> 5))
 __device__ __forceinline__ constexpr int reg_row(int r) { return (r & 3) + 8 * (r >> 2); }
 
@@ -311,9 +316,18 @@ attn_fwd_kernel(AttnArgs a) {
     auto tile = [&](const char* Ks, const char* Vs, int key0) {
         f32x16 s[2] = {{0}, {0}};
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+        for (int part = 0; part < DP / 64; ++part) {
+            x8 f[2][4];
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) s[sub] = mma(T::row(Ks, at, sub * 32, ks), qf[ks], s[sub]);
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) f[sub][ks] = T::row(Ks, at, sub * 32, 4 * part + ks);
+            reads_first();
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) s[sub] = mma(f[sub][ks], qf[4 * part + ks], s[sub]);
+        }
         if (key0 + kStage > seen_lo) {  // wave-uniform: some pair of the tile is not visible
             keep_branch();
             const int lim = seen - key0;
@@ -339,6 +353,12 @@ attn_fwd_kernel(AttnArgs a) {
         }
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
+            x8 vf[2][NB];
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int i = 0; i < NB; ++i) vf[g][i] = T::tr(Vs, at, sub * 32 + 16 * g, i);
+            reads_first();
             float r0 = 0.f, r1 = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
@@ -358,8 +378,8 @@ attn_fwd_kernel(AttnArgs a) {
             const x8 p0 = pack8<E>(s[sub], 0), p1 = pack8<E>(s[sub], 8);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                o[i] = mma(T::tr(Vs, at, sub * 32, i), p0, o[i]);
-                o[i] = mma(T::tr(Vs, at, sub * 32 + 16, i), p1, o[i]);
+                o[i] = mma(vf[0][i], p0, o[i]);
+                o[i] = mma(vf[1][i], p1, o[i]);
             }
         }
     };
@@ -751,10 +771,26 @@ attn_dq_kernel(AttnArgs a) {
     auto tile = [&](const char* Ks, const char* Vs, int key0) {
         f32x16 s = {0}, dp = {0};
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-            s = mma(T::row(Ks, at, 0, ks), qf[ks], s);
-            dp = mma(T::row(Vs, at, 0, ks), df[ks], dp);
+        for (int part = 0; part < DP / 64; ++part) {
+            x8 f[4], e[4];
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                f[ks] = T::row(Ks, at, 0, 4 * part + ks);
+                e[ks] = T::row(Vs, at, 0, 4 * part + ks);
+            }
+            reads_first();
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                s = mma(f[ks], qf[4 * part + ks], s);
+                dp = mma(e[ks], df[4 * part + ks], dp);
+            }
         }
+        x8 kt[2][NB];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) kt[g][i] = T::tr(Ks, at, 16 * g, i);
+        reads_first();
         unsigned w[4];
         if (kDrop) mask_bytes<true>(w, a.seed, head, step, key0, q0, lane);
 #pragma unroll
@@ -782,9 +818,8 @@ attn_dq_kernel(AttnArgs a) {
             const x8 ds = pack8<E>(dp, 8 * g), p = pack8<E>(s, 8 * g);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                const x8 k = T::tr(Ks, at, 16 * g, i);
-                dq[i] = mma(k, ds, dq[i]);
-                pk[i] = mma(k, p, pk[i]);
+                dq[i] = mma(kt[g][i], ds, dq[i]);
+                pk[i] = mma(kt[g][i], p, pk[i]);
             }
         }
     };
@@ -890,10 +925,29 @@ attn_dkdv_kernel(AttnArgs a) {
         auto tile = [&](const char* Qs, const char* Ds, const float* lse2, const float* del, int qs0) {
             f32x16 s = {0}, dp = {0};
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                s = mma(T::row(Qs, at, 0, ks), kf[ks], s);
-                dp = mma(T::row(Ds, at, 0, ks), vf[ks], dp);
+            for (int part = 0; part < DP / 64; ++part) {
+                x8 f[4], e[4];
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    f[ks] = T::row(Qs, at, 0, 4 * part + ks);
+                    e[ks] = T::row(Ds, at, 0, 4 * part + ks);
+                }
+                reads_first();
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    s = mma(f[ks], kf[4 * part + ks], s);
+                    dp = mma(e[ks], vf[4 * part + ks], dp);
+                }
             }
+            x8 qt[2][NB], dt[2][NB];
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    qt[g][i] = T::tr(Qs, at, 16 * g, i);
+                    dt[g][i] = T::tr(Ds, at, 16 * g, i);
+                }
+            reads_first();
             unsigned w[4];
             if (kDrop) mask_bytes<false>(w, a.seed, head, step, qs0, key0, lane);
 #pragma unroll
@@ -930,8 +984,8 @@ attn_dkdv_kernel(AttnArgs a) {
                 const x8 p = pack8<E>(pd, 8 * k), ds = pack8<E>(dp, 8 * k);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
-                    dv[i] = mma(p, T::tr(Ds, at, 16 * k, i), dv[i]);
-                    dk[i] = mma(ds, T::tr(Qs, at, 16 * k, i), dk[i]);
+                    dv[i] = mma(p, dt[k][i], dv[i]);
+                    dk[i] = mma(ds, qt[k][i], dk[i]);
                 }
             }
         };

@@ -83,8 +83,9 @@ struct AttnArgs {
     int B, Tq, Tk, H, Hk, D, causal;
     float scale, up;
     unsigned limit, step;
-    float* parts;             // few queries: partial results of the key chunks
+    float* parts;             // partial results of key chunks (few queries) or query ranges (dK / dV)
     int target;               // few queries: workgroups to cut the keys for (0: not cut)
+    int splits;               // dK / dV: query ranges
 };
 
 // -- tiles ------------------------------------------------------------------------------------
@@ -870,7 +871,10 @@ attn_dq_kernel(AttnArgs a) {
 
 // ---------------------------------------------------------------------------------------------
 // Backward, keys: one workgroup = 128 keys of one key head; streams Q / dO of every query head
-// that reads them.
+// that reads them.  Where that makes too few workgroups (few sequences, shared heads) the stages of
+// all heads are cut into `splits` ranges, one workgroup each (blockIdx.z): they leave fp32 sums in
+// `parts` ([range][dK, dV][B][Hk][Tk][DP]) that attn_add_kernel adds in order.  (6 ragged sequences
+// of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 66 + 10 us in four times as many.)
 template <class E, int DP, bool kDrop>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dkdv_kernel(AttnArgs a) {
@@ -899,8 +903,13 @@ attn_dkdv_kernel(AttnArgs a) {
     constexpr int kBuf = 2 * T::kBytes + 2 * R * 4;
     typename T::Regs qr, dr;
     float ls = 0.f, de = 0.f;
+    const int per = max(0, stages - first);
+    const int it0 = static_cast<int>(static_cast<long>(per) * group * blockIdx.z / a.splits);
+    const int it1 = static_cast<int>(static_cast<long>(per) * group * (blockIdx.z + 1) / a.splits);
     for (int g = 0; g < group; ++g) {
         const int h = hk * group + g;
+        const int lo = first + max(0, it0 - g * per), hi = first + min(per, it1 - g * per);  // stages of this head
+        if (lo >= hi) continue;
         const typename T::From qfrom = T::from(a.q, b * a.sq.b + h * a.sq.h, a.sq.t, sq.m, a.D, tid);
         const typename T::From dfrom = T::from(a.dout, b * a.sdo.b + h * a.sdo.h, a.sdo.t, sq.m, a.D, tid);
         const long rows = (static_cast<long>(b) * a.H + h) * a.Tq;
@@ -990,7 +999,7 @@ attn_dkdv_kernel(AttnArgs a) {
             }
         };
         auto stage = [&](int st, char* here, char* there) {
-            if (st + 1 < stages) fetch(st + 1);
+            if (st + 1 < hi) fetch(st + 1);
             const float* lse2 = reinterpret_cast<const float*>(here + 2 * T::kBytes);
 #pragma unroll
             for (int sub = 0; sub < R / 32; ++sub) {
@@ -1000,22 +1009,36 @@ attn_dkdv_kernel(AttnArgs a) {
                     tile(here + sub * 32 * T::kRow, here + T::kBytes + sub * 32 * T::kRow, lse2 + sub * 32,
                          lse2 + R + sub * 32, qs0);
             }
-            if (st + 1 < stages) fill(there);
+            if (st + 1 < hi) fill(there);
             __syncthreads();
         };
-        if (first < stages) {
-            fetch(first);
-            fill(smem);
-        }
+        fetch(lo);
+        fill(smem);
         __syncthreads();
-        for (int st = first; st < stages; st += 2) {
+        for (int st = lo; st < hi; st += 2) {
             stage(st, smem, smem + kBuf);
-            if (st + 1 < stages) stage(st + 1, smem + kBuf, smem);
+            if (st + 1 < hi) stage(st + 1, smem + kBuf, smem);
         }
     }
     // register r of block i: key key0 + acc_row(r), column 32 i + n.  (The factor of what is kept
     // comes last: the probabilities are rounded without it, so that a probability of 1 stays exact.)
     const float up = kDrop ? a.up : 1.f;
+    if (a.splits > 1) {
+        const long heads = static_cast<long>(a.B) * a.Hk;
+        float* pk = a.parts + ((2L * blockIdx.z * heads + bh) * a.Tk) * DP;
+        float* pv = pk + heads * a.Tk * DP;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = key0 + acc_row(r, lane);
+            if (j >= sq.n) continue;  // (not read)
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                pk[static_cast<long>(j) * DP + 32 * i + n] = dk[i][r] * a.scale;
+                pv[static_cast<long>(j) * DP + 32 * i + n] = dv[i][r] * up;
+            }
+        }
+        return;
+    }
     E* dkb = static_cast<E*>(a.dk) + b * a.sdk.b + hk * a.sdk.h;
     E* dvb = static_cast<E*>(a.dv) + b * a.sdv.b + hk * a.sdv.h;
 #pragma unroll
@@ -1031,6 +1054,36 @@ attn_dkdv_kernel(AttnArgs a) {
             dvb[j * a.sdv.t + c] = static_cast<E>(in ? dv[i][r] * up : 0.f);
         }
     }
+}
+
+// The ranges of attn_dkdv_kernel in order.  A thread takes four columns of a key's dK or dV.
+template <class E, int DP>
+__global__ void __launch_bounds__(256) attn_add_kernel(AttnArgs a) {
+    const long heads = static_cast<long>(a.B) * a.Hk, one = heads * a.Tk * DP;
+    const long at = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (at >= 2 * one) return;
+    const bool v = at >= one;
+    const long e = v ? at - one : at, row = e / DP;
+    const int c = static_cast<int>(e % DP), j = static_cast<int>(row % a.Tk);
+    const int b = static_cast<int>(row / a.Tk / a.Hk), hk = static_cast<int>(row / a.Tk % a.Hk);
+    if (c >= a.D) return;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (j < sequence(a, b).n) {
+        const float* p = a.parts + at;
+        for (int z0 = 0; z0 < a.splits; z0 += 4) {
+            f32x4 x[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z)
+                x[z] = z0 + z < a.splits ? *reinterpret_cast<const f32x4*>(p + 2 * one * (z0 + z)) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int z = 0; z < 4; ++z) sum += x[z];
+        }
+    }
+    typename Vec<E>::x4 out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = static_cast<E>(sum[i]);
+    const Strides& st = v ? a.sdv : a.sdk;
+    *reinterpret_cast<typename Vec<E>::x4*>(static_cast<E*>(v ? a.dv : a.dk) + b * st.b + j * st.t + hk * st.h + c) = out;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1072,6 +1125,19 @@ int launch_few(const AttnArgs& a, hipStream_t s) {
     return static_cast<int>(hipGetLastError());
 }
 
+// Query ranges of the dK / dV kernel: about two rounds of workgroups, while a range keeps six
+// stages (the sums of the ranges cost a launch and their way through memory) and there are at most
+// eight.
+int key_splits(const AttnArgs& a) {
+    const long groups = static_cast<long>(a.B) * a.Hk * ((a.Tk + 127) / 128);
+    const int wide = a.D > 64, rows = wide ? kBwdStage<128> : kBwdStage<64>;
+    const long most = static_cast<long>(a.H / a.Hk) * ((a.Tq + rows - 1) / rows) / 6;
+    const long want = ((wide ? 512 : 1024) + groups - 1) / groups;
+    const long n = want < most ? want : most;
+    return static_cast<int>(n < 1 ? 1 : n > 8 ? 8 : n);
+}
+long delta_floats(const AttnArgs& a) { return (static_cast<long>(a.B) * a.H * a.Tq + 3) & ~3L; }
+
 template <class E, int DP, bool kDrop>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {
     constexpr int rows = kBwdStage<DP>;
@@ -1079,7 +1145,11 @@ int launch_bwd(const AttnArgs& a, hipStream_t s) {
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop>), lds)) return st;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_dkdv_kernel<E, DP, kDrop>), lds2)) return st;
     hipLaunchKernelGGL((attn_dq_kernel<E, DP, kDrop>), dim3(a.B * a.H, (a.Tq + 127) / 128), dim3(256), lds, s, a);
-    hipLaunchKernelGGL((attn_dkdv_kernel<E, DP, kDrop>), dim3(a.B * a.Hk, (a.Tk + 127) / 128), dim3(256), lds2, s, a);
+    hipLaunchKernelGGL((attn_dkdv_kernel<E, DP, kDrop>), dim3(a.B * a.Hk, (a.Tk + 127) / 128, a.splits), dim3(256),
+                       lds2, s, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL((attn_add_kernel<E, DP>),
+                           dim3(static_cast<unsigned>((2L * a.B * a.Hk * a.Tk * DP / 4 + 255) / 256)), dim3(256), 0, s, a);
     return static_cast<int>(hipGetLastError());
 }
 
@@ -1108,8 +1178,16 @@ long nf_attention_fwd_floats(const AttnArgs* args) {
     return static_cast<long>(few_workgroups(a)) * a.Tq * (a.H / a.Hk) * (2 + padded_dim(a.D));
 }
 
+// ... and a backward call (args->delta)
+long nf_attention_bwd_floats(const AttnArgs* args) {
+    const AttnArgs& a = *args;
+    if (a.Hk <= 0 || a.Tk <= 0) return 0;
+    const int n = key_splits(a);
+    return delta_floats(a) + (n > 1 ? 2L * n * a.B * a.Hk * a.Tk * padded_dim(a.D) : 0);
+}
+
 // type: 1 bf16, 2 half.  backward 0: reads q, k, v and writes out, lse; 1: reads q, k, v, out,
-// lse, dout and writes dq, dk, dv (delta: B H Tq floats of scratch).
+// lse, dout and writes dq, dk, dv (delta: nf_attention_bwd_floats of scratch, 16-byte aligned).
 int nf_attention(const AttnArgs* args, int type, int backward, hipStream_t s) {
     AttnArgs a = *args;
     if (a.B <= 0 || a.H <= 0 || a.Hk <= 0 || a.Tq <= 0 || a.Tk <= 0 || a.H % a.Hk != 0) return -1;
@@ -1121,6 +1199,8 @@ int nf_attention(const AttnArgs* args, int type, int backward, hipStream_t s) {
                      !fits(a.dv, a.sdv) || a.delta == nullptr))
         return -2;
     a.target = backward ? -1 : few_target(a);
+    a.splits = backward ? key_splits(a) : 1;
+    if (backward) a.parts = a.delta + delta_floats(a);
     if (type == 1) return a.D <= 64 ? launch<bf16, 64>(a, backward, s) : launch<bf16, 128>(a, backward, s);
     if (type == 2) return a.D <= 64 ? launch<half, 64>(a, backward, s) : launch<half, 128>(a, backward, s);
     return -1;

@@ -35,6 +35,7 @@ _SIGS = {
     "nf_attn_set_split": ([I], None),
     "nf_attention_args_size": ([], I),
     "nf_attention_fwd_floats": ([P], L),
+    "nf_attention_bwd_floats": ([P], L),
     "nf_attention": ([P, I, I, P], I),
 }
 _fns: dict[str, object] = {}
@@ -135,7 +136,7 @@ _TYPES = {torch.bfloat16: 1, torch.float16: 2}
 # ``AttnArgs`` of csrc/hip/attention_general.hip: addresses (q k v out lse dout dq dk dv delta, the
 # lengths, the step in memory), distances between sequences, rows and heads (q k v out dout dq dk
 # dv), seed and first head, sizes, scale and factor of what is kept, threshold and step, scratch
-_PACK = struct.Struct("@13P24q2Q7i2f2IPi0q")
+_PACK = struct.Struct("@13P24q2Q7i2f2IP2i0q")
 _NONE = (0, 0, 0, 0)
 
 
@@ -152,7 +153,7 @@ class _Args:
             q[0], k[0], v[0], out[0], lse, dout[0], dq[0], dk[0], dv[0], delta, self.qlen, self.klen,
             self.step_at, *q[1:], *k[1:], *v[1:], *out[1:], *dout[1:], *dq[1:], *dk[1:], *dv[1:],
             self.seed, self.first_head, self.B, self.Tq, self.Tk, self.H, self.Hk, self.D, self.causal,
-            self.scale, self.up, self.limit, self.step, parts, 0)
+            self.scale, self.up, self.limit, self.step, parts, 0, 0)
 
 
 def _operand(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, written: bool) -> tuple:
@@ -319,9 +320,10 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
             t.copy_(g.view(a.B, a.Hk, a.H // a.Hk, a.Tk, a.D).sum(2).transpose(1, 2))
         return
     dev = q.device
-    delta = torch.empty(a.B * a.H * a.Tq, dtype=torch.float32, device=dev)
     with library.on_device(dev):
-        library.check(_fn("nf_attention")(a.pack(lse.data_ptr(), *operands, delta=delta.data_ptr()),
+        floats = _fn("nf_attention_bwd_floats")(a.pack(0, _NONE))
+        scratch = torch.empty(floats, dtype=torch.float32, device=dev)
+        library.check(_fn("nf_attention")(a.pack(lse.data_ptr(), *operands, delta=scratch.data_ptr()),
                                           _TYPES[q.dtype], 1, library.stream_ptr(dev)), "attention_bwd")
 
 

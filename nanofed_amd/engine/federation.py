@@ -433,7 +433,7 @@ class FederatedEngine:
         if cfg.model.startswith("gpt2") and on_gpu and cfg.dp is None and cfg.dtype == "bf16":
             m = self._host_model.cfg
             gpt2_ok = (
-                m.n_embd == 64 * m.n_head and m.dropout == 0.0 and cfg.seq_len % 128 == 0
+                m.n_embd == 64 * m.n_head and not m.drops() and cfg.seq_len % 128 == 0
                 and m.n_embd <= 2048
             )
         resnet_ok = False

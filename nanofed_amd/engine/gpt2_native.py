@@ -22,6 +22,13 @@ trainer runs the step by hand on flat buffers:
 
 Activations are bf16, statistics and losses fp32.
 
+Dropout (``GPT2Config.dropout`` / ``embd_dropout`` / ``resid_dropout``): no mask is stored; the
+kernels of ``ops.embedding``, ``ops.attention`` and ``ops.dropout`` draw it from (run seed, layer
+and kind, step, client and place), in the backward pass once more.  The step number is a device
+value of a captured step.  A client's masks do not depend on how the clients are grouped or placed.
+Attention with dropout, with another head dimension than 64, or (on a GPU) with sequences whose
+length is no multiple of 128 goes through ``ops.attention.attention_fwd`` / ``attention_bwd``.
+
 Clients.  With equal shards the clients of a GPU step together (``grouped``): their
 batches are stacked, every GEMM is ONE batched launch in which workgroup z reads
 client z's weights (``nf_gemm_bf16_batched``: a 4096-row layer GEMM alone makes 1.1
@@ -44,6 +51,8 @@ import torch.nn.functional as F
 from nanofed_amd.core.exceptions import DeviceError
 from nanofed_amd.models.gpt2 import GPT2Config
 from nanofed_amd.ops import attention as attn_ops
+from nanofed_amd.ops import dropout as drop_ops
+from nanofed_amd.ops import embedding as embed_ops
 from nanofed_amd.ops import gemm_ops
 from nanofed_amd.ops import group_ops as go
 from nanofed_amd.ops import nn_ops
@@ -69,6 +78,25 @@ WGRAD_STREAM = os.environ.get("NANOFED_GPT2_WGRAD_STREAM", "1") != "0"
 
 def _views(layout: ArenaLayout, flat: torch.Tensor) -> dict[str, torch.Tensor]:
     return {s.name: flat[s.offset : s.offset + s.numel].view(s.shape) for s in layout.segments}
+
+
+class _Masks:
+    """Which dropout masks a pass draws: the step number (or a device value that holds it) and the
+    client that the batch's first sequences belong to.  ``None`` in its place: no dropout."""
+
+    def __init__(self, trainer: "GPT2NativeTrainer", step: "int | torch.Tensor", client: int) -> None:
+        m = trainer.m
+        self.attn, self.embd, self.resid = m.dropout, m.embd_dropout, m.resid_dropout
+        self.run_seed, self.step, self.client = trainer.cfg.seed, step, client
+        self.batch = trainer.cfg.batch_size  # sequences that a client's range of masks has room for
+
+    def at(self, *site) -> dict:
+        return {"seed": drop_ops.site_seed(self.run_seed, *site), "step": self.step}
+
+    def rows(self, seq: int, width: int, *site, client: int = 0) -> dict:
+        """The same with the first element of a client's ``[batch * seq, width]`` (a short last
+        batch leaves the end of the range unused); ``client``: counted from the first one."""
+        return {"first": (self.client + client) * self.batch * seq * width, **self.at(*site)}
 
 
 class _Buffers:
@@ -102,6 +130,7 @@ class _Buffers:
         self.dact = bf(R, 4 * C)
         self.dqkv = bf(R, 3 * C)
         self.attn_scratch = attn_ops.backward_scratch(batch, m.n_head, seq, device)
+        self.dproj = bf(R, C) if m.resid_dropout else self.dres  # gradient behind the residual dropout
 
 
 class GPT2NativeTrainer(GroupTrainer):
@@ -115,10 +144,12 @@ class GPT2NativeTrainer(GroupTrainer):
     ) -> None:
         if cfg.dp is not None:
             raise DeviceError("the GPT-2 trainer has no DP-SGD path")
-        if model_cfg.dropout != 0.0:
-            raise DeviceError("the GPT-2 trainer does not implement dropout")
-        if model_cfg.n_embd % model_cfg.n_head or (model_cfg.n_embd // model_cfg.n_head) != 64:
-            raise DeviceError("the attention kernels need a head dimension of 64")
+        for p, bits in ((model_cfg.dropout, 8), (model_cfg.embd_dropout, 16), (model_cfg.resid_dropout, 16)):
+            drop_ops.limit_of(p, bits, "the GPT-2 trainer")
+        head_dim = model_cfg.n_embd // model_cfg.n_head
+        if model_cfg.n_embd % model_cfg.n_head or head_dim % 8 or head_dim > attn_ops.MAX_HEAD_DIM:
+            raise DeviceError("the attention kernels need a head dimension that is a multiple of 8 up to "
+                              f"{attn_ops.MAX_HEAD_DIM}")
         self.cfg, self.pool, self.shards, self.m = cfg, pool, shards, model_cfg
         self.layout = pool.layout
         self.device = pool.data.device
@@ -169,7 +200,10 @@ class GPT2NativeTrainer(GroupTrainer):
         # grouped steps: equal shards of full batches, one lane, the native GEMM path
         self.group = 0
         if (GROUP > 1 and G > 1 and self.lanes == 1 and self.native_gemm and full_batches
-                and self.device.type == "cuda" and len(set(shards.sizes)) == 1):
+                and self.device.type == "cuda" and len(set(shards.sizes)) == 1
+                # (one launch draws the masks of consecutive clients)
+                and (not model_cfg.drops() or shards.client_ids == list(range(
+                    shards.client_ids[0], shards.client_ids[0] + G)))):
             self.group = min(GROUP, G)
             self._ggrads = torch.zeros(self.group, n, dtype=BF16, device=self.device)
             self._gslabs = torch.empty(1, dtype=torch.float32, device=self.device)
@@ -214,15 +248,84 @@ class GPT2NativeTrainer(GroupTrainer):
         else:
             torch.mm(dy.t(), x, out=out)
 
+    # -- what dropout changes: the embedding, attention and the two projections -------------
+    def _masks(self, step: "int | torch.Tensor", k: int) -> _Masks | None:
+        """The masks of optimisation step ``step`` for client k of the pool and those behind it."""
+        return _Masks(self, step, self.shards.client_ids[k]) if self.m.drops() else None
+
+    def _step_number(self, round_idx: int, epoch: int, step: int) -> int:
+        per = max(self.shards.max_steps(), 1)
+        return ((round_idx * self.cfg.local_epochs + epoch) * per + step) & 0xFFFFFFFF
+
+    def _embed(self, tokens: torch.Tensor, w: dict[str, torch.Tensor], seq: int, out: torch.Tensor,
+               masks: _Masks | None, client: int = 0) -> None:
+        """``client``: counted from the first one of ``masks``."""
+        if masks is None or not masks.embd:
+            nn_ops.embed_fwd(tokens.reshape(-1), w["wte.weight"], w["wpe.weight"], seq, out=out)
+            return
+        embed_ops.embedding_fwd(tokens.view(-1, seq), w["wte.weight"], out, positions=w["wpe.weight"],
+                                dropout=masks.embd, **masks.rows(seq, out.shape[-1], "embd", client=client))
+
+    def _embed_bwd(self, tokens: torch.Tensor, dx: torch.Tensor, g: dict[str, torch.Tensor], batch: int,
+                   seq: int, masks: _Masks | None, client: int = 0, order: torch.Tensor | None = None) -> None:
+        if masks is None or not masks.embd:
+            nn_ops.embed_bwd(tokens, dx, g["wte.weight"], g["wpe.weight"], batch, seq,
+                             sorted_tokens=order[0] if order is not None else None,
+                             order=order[1] if order is not None else None)
+            return
+        embed_ops.embedding_bwd(tokens.view(batch, seq), dx, g["wte.weight"], dpositions=g["wpe.weight"],
+                                accumulate=True, dropout=masks.embd,
+                                **masks.rows(seq, dx.shape[-1], "embd", client=client))
+
+    def _attn_args(self, l: int, qkv: torch.Tensor, b: _Buffers, masks: _Masks | None):
+        hd = self.m.n_embd // self.m.n_head
+        drops = masks is not None and masks.attn > 0
+        if not drops and hd == attn_ops.HEAD_DIM and (qkv.device.type != "cuda" or b.seq % 128 == 0):
+            return None, None
+        how = dict(dropout=masks.attn, first_batch=masks.client * masks.batch, **masks.at("attn", l)) if drops else {}
+        return qkv.view(b.batch, b.seq, 3, self.m.n_head, hd).unbind(2), how
+
+    def _attention(self, l: int, b: _Buffers, masks: _Masks | None) -> None:
+        parts, how = self._attn_args(l, b.qkv[l], b, masks)
+        if parts is None:
+            attn_ops.causal_attention_fwd(b.qkv[l], b.att[l], b.lse[l], b.batch, b.seq, self.m.n_head)
+        else:
+            attn_ops.attention_fwd(*parts, b.att[l].view(parts[0].shape), b.lse[l], **how)
+
+    def _attention_bwd(self, l: int, b: _Buffers, masks: _Masks | None) -> None:
+        parts, how = self._attn_args(l, b.qkv[l], b, masks)
+        if parts is None:
+            attn_ops.causal_attention_bwd(b.qkv[l], b.att[l], b.lse[l], b.datt, b.dqkv, b.attn_scratch,
+                                          b.batch, b.seq, self.m.n_head)
+            return
+        shape = parts[0].shape
+        grads = b.dqkv.view(b.batch, b.seq, 3, *shape[2:]).unbind(2)
+        attn_ops.attention_bwd(*parts, b.att[l].view(shape), b.lse[l], b.datt.view(shape), *grads, **how)
+
+    def _resid(self, b: _Buffers, masks: _Masks | None, *site) -> torch.Tensor:
+        """Dropout of a projection's output (in place) before it joins the residual stream."""
+        if masks is not None and masks.resid:
+            drop_ops.dropout_fwd(b.tmp_c, masks.resid, out=b.tmp_c,
+                                 **masks.rows(b.seq, b.tmp_c.shape[1], *site))
+        return b.tmp_c
+
+    def _resid_bwd(self, b: _Buffers, masks: _Masks | None, *site) -> torch.Tensor:
+        """The gradient of the projection's output from that of the residual stream."""
+        if masks is None or not masks.resid:
+            return b.dres
+        return drop_ops.dropout_bwd(b.dres, masks.resid, out=b.dproj,
+                                    **masks.rows(b.seq, b.dres.shape[1], *site))
+
     # -- forward ------------------------------------------------------------
-    def _forward(self, w: dict[str, torch.Tensor], tokens: torch.Tensor, b: _Buffers) -> None:
+    def _forward(self, w: dict[str, torch.Tensor], tokens: torch.Tensor, b: _Buffers,
+                 masks: _Masks | None = None) -> None:
         """Fills the activation buffers and leaves d(logits) in ``b.logits``,
         per-row losses in ``b.loss_rows``."""
         m, L = self.m, self.m.n_layer
         inp = tokens[:, :-1].contiguous().view(-1)
         tgt = tokens[:, 1:].contiguous().view(-1)
         V = m.vocab_size
-        nn_ops.embed_fwd(inp, w["wte.weight"], w["wpe.weight"], b.seq, out=b.x[0])
+        self._embed(inp, w, b.seq, b.x[0], masks)
         delta = None
         for l in range(L):
             p = f"h.{l}."
@@ -234,14 +337,14 @@ class GPT2NativeTrainer(GroupTrainer):
                 nn_ops.ln_fwd(b.x_mid[l - 1], w[p + "ln_1.weight"], w[p + "ln_1.bias"],
                               b.ln1[l], st1[0], st1[1], delta=delta, x_out=b.x[l])
             self._lin_fwd(b.ln1[l], w[p + "attn.c_attn.weight"], w[p + "attn.c_attn.bias"], b.qkv[l])
-            attn_ops.causal_attention_fwd(b.qkv[l], b.att[l], b.lse[l], b.batch, b.seq, m.n_head)
+            self._attention(l, b, masks)
             self._lin_fwd(b.att[l], w[p + "attn.c_proj.weight"], w[p + "attn.c_proj.bias"], b.tmp_c)
             nn_ops.ln_fwd(b.x[l], w[p + "ln_2.weight"], w[p + "ln_2.bias"], b.ln2[l],
-                          st2[0], st2[1], delta=b.tmp_c, x_out=b.x_mid[l])
+                          st2[0], st2[1], delta=self._resid(b, masks, "attn_proj", l), x_out=b.x_mid[l])
             self._lin_fwd(b.ln2[l], w[p + "c_fc.weight"], w[p + "c_fc.bias"], b.fc[l],
                           gelu_out=b.act[l])
             self._lin_fwd(b.act[l], w[p + "c_proj.weight"], w[p + "c_proj.bias"], b.tmp_c)
-            delta = b.tmp_c
+            delta = self._resid(b, masks, "proj", l)
         stf = b.stats[2 * L]
         nn_ops.ln_fwd(b.x_mid[L - 1], w["ln_f.weight"], w["ln_f.bias"], b.lnf, stf[0], stf[1],
                       delta=delta, x_out=b.x[L])
@@ -250,8 +353,19 @@ class GPT2NativeTrainer(GroupTrainer):
 
     # -- backward -----------------------------------------------------------
     def _backward(self, w: dict[str, torch.Tensor], tokens: torch.Tensor, b: _Buffers,
-                  g: dict[str, torch.Tensor]) -> None:
+                  g: dict[str, torch.Tensor], masks: _Masks | None = None) -> None:
         m, L = self.m, self.m.n_layer
+        resid = masks is not None and masks.resid > 0
+
+        def joined(name):
+            # with residual dropout the projection's bias gradient is not the column sum of d(x)
+            return None if resid else g[name]
+
+        def proj_bwd(name, *site):
+            d = self._resid_bwd(b, masks, *site)
+            if resid:
+                nn_ops.colsum(d, g[name])
+            return d
         V = m.vocab_size
         dlog = b.logits[:, :V]
         self._lin_wgrad(dlog, b.lnf, g["wte.weight"])  # LM head shares the embedding matrix
@@ -260,40 +374,41 @@ class GPT2NativeTrainer(GroupTrainer):
         # every LayerNorm backward also sums its d(x) over the rows: that is the bias
         # gradient of the projection that wrote into the residual stream before it
         nn_ops.ln_bwd(b.dln, b.x[L], w["ln_f.weight"], stf[0], stf[1], b.dres,
-                      g["ln_f.weight"], g["ln_f.bias"], dxsum=g[f"h.{L - 1}.c_proj.bias"])
+                      g["ln_f.weight"], g["ln_f.bias"], dxsum=joined(f"h.{L - 1}.c_proj.bias"))
         for l in reversed(range(L)):
             p = f"h.{l}."
             st1, st2 = b.stats[2 * l], b.stats[2 * l + 1]
             # MLP: x_next = x_mid + c_proj(gelu(c_fc(ln_2(x_mid))))
-            self._lin_wgrad(b.dres, b.act[l], g[p + "c_proj.weight"])
-            self._lin_dgrad(b.dres, w[p + "c_proj.weight"], b.dact)
+            d = proj_bwd(p + "c_proj.bias", "proj", l)
+            self._lin_wgrad(d, b.act[l], g[p + "c_proj.weight"])
+            self._lin_dgrad(d, w[p + "c_proj.weight"], b.dact)
             nn_ops.gelu_bwd_colsum(b.fc[l], b.dact, b.dact, g[p + "c_fc.bias"])
             self._lin_wgrad(b.dact, b.ln2[l], g[p + "c_fc.weight"])
             self._lin_dgrad(b.dact, w[p + "c_fc.weight"], b.dln)
             nn_ops.ln_bwd(b.dln, b.x_mid[l], w[p + "ln_2.weight"], st2[0], st2[1], b.dres,
                           g[p + "ln_2.weight"], g[p + "ln_2.bias"], dres=b.dres,
-                          dxsum=g[p + "attn.c_proj.bias"])
+                          dxsum=joined(p + "attn.c_proj.bias"))
             # attention: x_mid = x + c_proj(attn(c_attn(ln_1(x))))
-            self._lin_wgrad(b.dres, b.att[l], g[p + "attn.c_proj.weight"])
-            self._lin_dgrad(b.dres, w[p + "attn.c_proj.weight"], b.datt)
-            attn_ops.causal_attention_bwd(b.qkv[l], b.att[l], b.lse[l], b.datt, b.dqkv,
-                                          b.attn_scratch, b.batch, b.seq, m.n_head)
+            d = proj_bwd(p + "attn.c_proj.bias", "attn_proj", l)
+            self._lin_wgrad(d, b.att[l], g[p + "attn.c_proj.weight"])
+            self._lin_dgrad(d, w[p + "attn.c_proj.weight"], b.datt)
+            self._attention_bwd(l, b, masks)
             nn_ops.colsum(b.dqkv, g[p + "attn.c_attn.bias"])
             self._lin_wgrad(b.dqkv, b.ln1[l], g[p + "attn.c_attn.weight"])
             self._lin_dgrad(b.dqkv, w[p + "attn.c_attn.weight"], b.dln)
             nn_ops.ln_bwd(b.dln, b.x[l], w[p + "ln_1.weight"], st1[0], st1[1], b.dres,
                           g[p + "ln_1.weight"], g[p + "ln_1.bias"], dres=b.dres,
-                          dxsum=g[f"h.{l - 1}.c_proj.bias"] if l > 0 else None)
-        nn_ops.embed_bwd(tokens[:, :-1].contiguous(), b.dres, g["wte.weight"], g["wpe.weight"],
-                         b.batch, b.seq)
+                          dxsum=joined(f"h.{l - 1}.c_proj.bias") if l > 0 else None)
+        self._embed_bwd(tokens[:, :-1].contiguous(), b.dres, g, b.batch, b.seq, masks)
 
     # -- one optimisation step of client k ------------------------------------
-    def _step(self, k: int, tokens: torch.Tensor, lane: int = 0) -> None:
+    def _step(self, k: int, tokens: torch.Tensor, lane: int = 0, number: int = 0) -> None:
         cfg = self.cfg
         b = self._buffers(tokens.shape[0], tokens.shape[1] - 1, lane)
         w = _views(self.layout, self.shadow[k])
-        self._forward(w, tokens, b)
-        self._backward(w, tokens, b, self._gvs[lane])
+        masks = self._masks(number, k)
+        self._forward(w, tokens, b, masks)
+        self._backward(w, tokens, b, self._gvs[lane], masks)
         nn_ops.sgd_step_bf16g(self.pool[k].data, self._grads[lane], self.shadow[k],
                               cfg.learning_rate, cfg.weight_decay)
         acc = self._acc[k]
@@ -301,14 +416,17 @@ class GPT2NativeTrainer(GroupTrainer):
         acc[1] += b.correct_rows.mean()
         acc[2] += 1.0
 
-    def loss_and_grads(self, k: int, tokens: torch.Tensor) -> tuple[float, dict[str, torch.Tensor]]:
+    def loss_and_grads(self, k: int, tokens: torch.Tensor, number: int = 0
+                       ) -> tuple[float, dict[str, torch.Tensor]]:
         """Loss and the flat gradient views of one batch, without an update
-        (the kernel tests compare these with autograd)."""
+        (the kernel tests compare these with autograd).  ``number``: the step whose dropout masks
+        are drawn."""
         b = self._buffers(tokens.shape[0], tokens.shape[1] - 1)
         self.shadow[k].copy_(self.pool[k].data)
         w = _views(self.layout, self.shadow[k])
-        self._forward(w, tokens, b)
-        self._backward(w, tokens, b, self._gvs[0])
+        masks = self._masks(number, k)
+        self._forward(w, tokens, b, masks)
+        self._backward(w, tokens, b, self._gvs[0], masks)
         return float(b.loss_rows.mean()), self._gvs[0]
 
     # -- grouped step: clients g0 .. g0 + Gn - 1 together ---------------------------------
@@ -387,11 +505,12 @@ class GPT2NativeTrainer(GroupTrainer):
         main.wait_event(done)
 
     def _gstep(self, g0: int, Gn: int, tokens: torch.Tensor,
-               order: torch.Tensor | None = None) -> None:
+               order: torch.Tensor | None = None, number: "int | torch.Tensor" = 0) -> None:
         """One optimisation step of Gn clients; ``tokens`` ``[Gn * batch, seq + 1]``,
         client-major.  ``order`` ``[Gn, 2, batch * seq]``: per client the sorted input tokens
         and their stable sort order (drawn on the host with the batch); without it the
-        embedding gradient sorts on the device."""
+        embedding gradient sorts on the device.  ``number``: the step's number for the dropout
+        masks, or one int64 on the device that holds it."""
         cfg, m, L = self.cfg, self.m, self.m.n_layer
         nb = tokens.shape[0] // Gn                       # sequences per client
         b = self._buffers(tokens.shape[0], tokens.shape[1] - 1, lane=100 + Gn)
@@ -402,6 +521,9 @@ class GPT2NativeTrainer(GroupTrainer):
         inp = tokens[:, :-1].contiguous()
         tgt = tokens[:, 1:].contiguous().view(-1)
         flat_inp = inp.view(-1)
+
+        masks = self._masks(number, g0)
+        resid = masks is not None and masks.resid > 0
 
         def wref(name):      # bf16 parameter copy of the group's first client
             return Ref(self.shadow[g0:], self._off(name))
@@ -415,8 +537,7 @@ class GPT2NativeTrainer(GroupTrainer):
 
         # forward
         for j in range(Gn):
-            nn_ops.embed_fwd(flat_inp[rows[j]], ws[j]["wte.weight"], ws[j]["wpe.weight"], b.seq,
-                             out=b.x[0][rows[j]])
+            self._embed(flat_inp[rows[j]], ws[j], b.seq, b.x[0][rows[j]], masks, j)
         delta = None
         for l in range(L):
             p = f"h.{l}."
@@ -427,14 +548,15 @@ class GPT2NativeTrainer(GroupTrainer):
                 ln(b.x_mid[l - 1], p + "ln_1", b.ln1[l], st1, delta=delta, x_out=b.x[l])
             self._glin_fwd(b.ln1[l], p + "attn.c_attn.weight", p + "attn.c_attn.bias", b.qkv[l],
                            g0, Gn, R)
-            attn_ops.causal_attention_fwd(b.qkv[l], b.att[l], b.lse[l], b.batch, b.seq, m.n_head)
+            self._attention(l, b, masks)
             self._glin_fwd(b.att[l], p + "attn.c_proj.weight", p + "attn.c_proj.bias", b.tmp_c,
                            g0, Gn, R)
-            ln(b.x[l], p + "ln_2", b.ln2[l], st2, delta=b.tmp_c, x_out=b.x_mid[l])
+            ln(b.x[l], p + "ln_2", b.ln2[l], st2, delta=self._resid(b, masks, "attn_proj", l),
+               x_out=b.x_mid[l])
             self._glin_fwd(b.ln2[l], p + "c_fc.weight", p + "c_fc.bias", b.fc[l], g0, Gn, R,
                            gelu_out=b.act[l])
             self._glin_fwd(b.act[l], p + "c_proj.weight", p + "c_proj.bias", b.tmp_c, g0, Gn, R)
-            delta = b.tmp_c
+            delta = self._resid(b, masks, "proj", l)
         stf = b.stats[2 * L]
         ln(b.x_mid[L - 1], "ln_f", b.lnf, stf, delta=delta, x_out=b.x[L])
         self._glin_fwd(b.lnf, "wte.weight", None, b.logits, g0, Gn, R, n_out=V)
@@ -444,29 +566,33 @@ class GPT2NativeTrainer(GroupTrainer):
         def ln_b(dy, x, name, st, dres=None, dxsum=None):
             nn_ops.ln_bwd_g(dy, x, wref(name + ".weight"), st[0], st[1], b.dres,
                             gref(name + ".weight"), gref(name + ".bias"), Gn, dres=dres,
-                            dxsum=gref(dxsum) if dxsum is not None else None)
+                            dxsum=gref(dxsum) if dxsum is not None and not resid else None)
+
+        def proj_bwd(name, *site):
+            """(gradient of a projection's output, its bias gradient where no LayerNorm made it)"""
+            d = self._resid_bwd(b, masks, *site)
+            return d, (lambda: nn_ops.colsum_g(d, gref(name), Gn)) if resid else None
 
         self._glin_bwd(b.logits, b.lnf, "wte.weight", b.dln, g0, Gn, R, n=V)
         ln_b(b.dln, b.x[L], "ln_f", stf, dxsum=f"h.{L - 1}.c_proj.bias")
         for l in reversed(range(L)):
             p = f"h.{l}."
             st1, st2 = b.stats[2 * l], b.stats[2 * l + 1]
-            self._glin_bwd(b.dres, b.act[l], p + "c_proj.weight", b.dact, g0, Gn, R)
+            d, bias = proj_bwd(p + "c_proj.bias", "proj", l)
+            self._glin_bwd(d, b.act[l], p + "c_proj.weight", b.dact, g0, Gn, R, also=bias)
             nn_ops.gelu_bwd_colsum_g(b.fc[l], b.dact, b.dact, gref(p + "c_fc.bias"), Gn)
             self._glin_bwd(b.dact, b.ln2[l], p + "c_fc.weight", b.dln, g0, Gn, R)
             ln_b(b.dln, b.x_mid[l], p + "ln_2", st2, dres=b.dres, dxsum=p + "attn.c_proj.bias")
-            self._glin_bwd(b.dres, b.att[l], p + "attn.c_proj.weight", b.datt, g0, Gn, R)
-            attn_ops.causal_attention_bwd(b.qkv[l], b.att[l], b.lse[l], b.datt, b.dqkv,
-                                          b.attn_scratch, b.batch, b.seq, m.n_head)
+            d, bias = proj_bwd(p + "attn.c_proj.bias", "attn_proj", l)
+            self._glin_bwd(d, b.att[l], p + "attn.c_proj.weight", b.datt, g0, Gn, R, also=bias)
+            self._attention_bwd(l, b, masks)
             self._glin_bwd(b.dqkv, b.ln1[l], p + "attn.c_attn.weight", b.dln, g0, Gn, R,
                            also=lambda p=p: nn_ops.colsum_g(b.dqkv, gref(p + "attn.c_attn.bias"), Gn))
             ln_b(b.dln, b.x[l], p + "ln_1", st1, dres=b.dres,
                  dxsum=f"h.{l - 1}.c_proj.bias" if l > 0 else None)
         for j in range(Gn):
-            nn_ops.embed_bwd(inp[j * nb : (j + 1) * nb], b.dres[rows[j]], gs[j]["wte.weight"],
-                             gs[j]["wpe.weight"], nb, b.seq,
-                             sorted_tokens=order[j, 0] if order is not None else None,
-                             order=order[j, 1] if order is not None else None)
+            self._embed_bwd(inp[j * nb : (j + 1) * nb], b.dres[rows[j]], gs[j], nb, b.seq, masks, j,
+                            order[j] if order is not None else None)
         n = self.layout.numel
         nn_ops.sgd_step_bf16g(self.pool.data[g0 : g0 + Gn].view(-1), self._ggrads[:Gn].view(-1),
                               self.shadow[g0 : g0 + Gn].view(-1), cfg.learning_rate,
@@ -490,7 +616,8 @@ class GPT2NativeTrainer(GroupTrainer):
                 for g0 in range(0, G, self.group):
                     Gn = min(self.group, G - g0)
                     rows = perms[g0 : g0 + Gn, s].reshape(-1)
-                    self._gstep(g0, Gn, self.shards.inputs[rows])
+                    self._gstep(g0, Gn, self.shards.inputs[rows],
+                                number=self._step_number(round_idx, epoch, s))
 
     def _train_round_graphs(self, round_idx: int, steps: int) -> None:
         """The grouped step as one hipGraph replay per step and group.  What changes from
@@ -511,6 +638,8 @@ class GPT2NativeTrainer(GroupTrainer):
         # the round's batches, in page-locked memory: [epoch, step, client] blocks
         tok = torch.empty(E, steps, G * B, S1, dtype=torch.int64).pin_memory()
         order = torch.empty(E, steps, G, 2, B * (S1 - 1), dtype=torch.int64).pin_memory()
+        number = torch.tensor([[self._step_number(round_idx, e, s) for s in range(steps)]
+                               for e in range(E)], dtype=torch.int64).pin_memory()
         for epoch in range(E):
             perms = torch.stack([self.shards.host_permutation(k, round_idx, epoch)
                                  for k in range(G)]).view(G, steps, B)
@@ -528,17 +657,19 @@ class GPT2NativeTrainer(GroupTrainer):
                     st = self._static_inputs(g0, Gn, S1)
                     st["tokens"].copy_(tok[epoch, s, g0 * B : (g0 + Gn) * B], non_blocking=True)
                     st["order"].copy_(order[epoch, s, g0 : g0 + Gn], non_blocking=True)
+                    if self.m.drops():
+                        st["number"].copy_(number[epoch, s], non_blocking=True)
                     graph = self._step_graphs.get((g0, Gn))
                     if graph is None and st["warm"]:
                         torch.cuda.synchronize(self.device)
                         graph = torch.cuda.CUDAGraph()
                         with torch.cuda.graph(graph):
-                            self._gstep(g0, Gn, st["tokens"], st["order"])
+                            self._gstep(g0, Gn, st["tokens"], st["order"], st["number"])
                         self._step_graphs[(g0, Gn)] = graph
                     if graph is not None:
                         graph.replay()
                     else:
-                        self._gstep(g0, Gn, st["tokens"], st["order"])
+                        self._gstep(g0, Gn, st["tokens"], st["order"], st["number"])
                         st["warm"] = True
 
     def _static_inputs(self, g0: int, Gn: int, S1: int) -> dict:
@@ -548,6 +679,7 @@ class GPT2NativeTrainer(GroupTrainer):
             self._step_inputs[key] = {
                 "tokens": torch.zeros(Gn * B, S1, dtype=torch.int64, device=self.device),
                 "order": torch.zeros(Gn, 2, B * (S1 - 1), dtype=torch.int64, device=self.device),
+                "number": torch.zeros((), dtype=torch.int64, device=self.device),
                 "warm": False,
             }
         return self._step_inputs[key]
@@ -580,16 +712,17 @@ class GPT2NativeTrainer(GroupTrainer):
                             continue
                         lane = k % self.lanes
                         lo = s * cfg.batch_size
+                        number = self._step_number(round_idx, epoch, s)
                         rows = perms[k][epoch][lo : lo + cfg.batch_size]
                         if self._streams:
                             with torch.cuda.stream(self._streams[lane]):
                                 if s == 0:
                                     self._acc[k].zero_()
-                                self._step(k, self.shards.inputs[rows], lane)
+                                self._step(k, self.shards.inputs[rows], lane, number)
                         else:
                             if s == 0:
                                 self._acc[k].zero_()
-                            self._step(k, self.shards.inputs[rows], lane)
+                            self._step(k, self.shards.inputs[rows], lane, number)
         if self._streams:
             for st in self._streams:
                 main.wait_stream(st)

@@ -5,6 +5,10 @@ Used for the large-arena federated configuration, where the cost of a round
 is dominated by the size of the parameter reduce.  Attention goes through
 ``scaled_dot_product_attention`` (flash kernel on ROCm); the token embedding
 and the LM head share one weight, so the arena holds it once.
+
+``dropout`` drops attention probabilities, ``embd_dropout`` the sum of the two
+embeddings, ``resid_dropout`` the output of both projections of a block before it
+is added to the residual stream.  All are 0 by default.
 """
 
 from __future__ import annotations
@@ -25,6 +29,12 @@ class GPT2Config:
     n_layer: int = 12
     n_head: int = 12
     dropout: float = 0.0
+    embd_dropout: float = 0.0
+    resid_dropout: float = 0.0
+
+    def drops(self) -> bool:
+        """Whether a training step draws dropout masks."""
+        return max(self.dropout, self.embd_dropout, self.resid_dropout) > 0.0
 
 
 class _Attention(nn.Module):
@@ -57,11 +67,15 @@ class _Block(nn.Module):
         self.ln_2 = nn.LayerNorm(cfg.n_embd)
         self.c_fc = nn.Linear(cfg.n_embd, 4 * cfg.n_embd)
         self.c_proj = nn.Linear(4 * cfg.n_embd, cfg.n_embd)
+        self.dropout = cfg.resid_dropout
+
+    def _drop(self, x: torch.Tensor) -> torch.Tensor:
+        return F.dropout(x, self.dropout, self.training) if self.dropout else x
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x = x + self.attn(self.ln_1(x))
+        x = x + self._drop(self.attn(self.ln_1(x)))
         h = F.gelu(self.c_fc(self.ln_2(x)), approximate="tanh")
-        return x + self.c_proj(h)
+        return x + self._drop(self.c_proj(h))
 
 
 class GPT2LM(nn.Module):
@@ -92,6 +106,8 @@ class GPT2LM(nn.Module):
         _, t = idx.shape
         pos = torch.arange(t, device=idx.device)
         x = self.wte(idx) + self.wpe(pos)
+        if self.cfg.embd_dropout:
+            x = F.dropout(x, self.cfg.embd_dropout, self.training)
         for block in self.h:
             x = block(x)
         return F.linear(self.ln_f(x), self.wte.weight)

@@ -15,6 +15,7 @@ also what the kernel tests compare against.  The reference applies ``F.dropout``
 
 from __future__ import annotations
 
+import hashlib
 from ctypes import c_int, c_long, c_uint, c_ulonglong, c_void_p
 
 import torch
@@ -41,6 +42,13 @@ def _fn(name: str):
 
 def symbols() -> list[str]:
     return sorted(_SIGS)
+
+
+def site_seed(seed: int, *site) -> int:
+    """A 64-bit seed for one place of a model (layer, kind of dropout) under a run's seed: places
+    with different names draw independent masks."""
+    text = "|".join(str(x) for x in (seed, *site))
+    return int.from_bytes(hashlib.sha256(text.encode()).digest()[:8], "little")
 
 
 # -- the generator ------------------------------------------------------------------------

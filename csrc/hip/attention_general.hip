@@ -436,9 +436,12 @@ attn_fwd_kernel(AttnArgs a) {
 // The chunks are cut on the device, from the lengths: about `target` of equal size over all
 // sequences, so a batch of short and long ones still fills the chip evenly.  What a chunk costs
 // apart from its keys (the first load, the joins) is worth some hundred keys, so there are no more
-// of them than workgroups run at once.  (Chunks of 256 / 1024 keys for every sequence measured
-// 28.7 / 23.8 us on four caches of up to 8191 keys x 8 heads x 128, equal shares of the 84 MB KTIME.)
-constexpr int kFew = 32, kFewMaxBatch = 512;
+// of them than workgroups run at once.  (Four caches of up to 8191 keys x 8 heads x 128, 84 MB:
+// 19.0 us + 5.4 us for the join with 512 workgroups, 4.4 TB/s; 23.0 + 4.9 with 256; without the
+// hint that the keys are read once, which leaves the parts in L2, 20.2 + 6.2.)
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+constexpr int kFew = 32, kFewMaxBatch = 512, kFewTarget = 512;
+constexpr int kOnce = 2;  // non-temporal load
 
 struct Chunk { int b, hk, count, at, size; Seq seq; };  // chunk `at` of `count` of (b, hk), keys per chunk
 
@@ -525,10 +528,10 @@ attn_few_kernel(AttnArgs a) {
             const_cast<E*>(vb + key0 * a.sv.t), 0, static_cast<int>((last * a.sv.t + a.D) * 2), 0x00020000);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(kd, static_cast<int>(koff[i]), 0, 0);
+            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(kd, static_cast<int>(koff[i]), 0, kOnce);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vd, static_cast<int>(voff[i]), 0, 0);
+            vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vd, static_cast<int>(voff[i]), 0, kOnce);
     };
     f32x16 o[NB];
 #pragma unroll
@@ -586,42 +589,16 @@ attn_few_kernel(AttnArgs a) {
         }
     }
     l = sum_halves(l);
-    // join the waves: 2, 3 into 0, 1, then 1 into 0
-    constexpr int kPark = 64 * (NB * 16 + 2);
-    float* park = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-            float* to = park + (wave - half) * kPark + lane;
-            to[0] = m;
-            to[64] = l;
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) to[64 * (2 + 16 * i + r)] = o[i][r];
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float* from = park + wave * kPark + lane;
-            const float m2 = from[0], l2 = from[64], mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
-            const float a1 = exp2_fast((m - ref) * sc2), a2 = exp2_fast((m2 - ref) * sc2);
-            m = mn;
-            l = l * a1 + l2 * a2;
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[i][r] = o[i][r] * a1 + from[64 * (2 + 16 * i + r)] * a2;
-        }
+    // Join the waves: each leaves its m, l and O [rows][DP] (where its tiles were; the 16-byte pieces
+    // of a row permuted, as a row is a whole number of bank rounds), then all threads sum them.
+    constexpr int kPieces = DP / 4;
+    float* ml = reinterpret_cast<float*>(smem + 8 * T::kBytes);  // [wave][m, l][32]
+    if (hh == 0) {
+        ml[wave * 64 + n] = m;
+        ml[wave * 64 + 32 + n] = l;
     }
-    if (wave != 0 || n >= rows) return;
-    if (me.count > 1) {
-        const long part = static_cast<long>(blockIdx.x) * rows + n, parts = static_cast<long>(gridDim.x) * rows;
-        if (hh == 0) {
-            a.parts[parts * DP + 2 * part] = m;
-            a.parts[parts * DP + 2 * part + 1] = l;
-        }
-        float* to = a.parts + part * DP;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (n < rows) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -629,26 +606,46 @@ attn_few_kernel(AttnArgs a) {
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = o[i][4 * g + e];
-                *reinterpret_cast<f32x4*>(to + 32 * i + 8 * g + 4 * hh) = v;
+                *reinterpret_cast<f32x4*>(lds + (n * kPieces + ((8 * i + 2 * g + hh) ^ (n & (kPieces - 1)))) * 16) = v;
             }
-        return;
     }
-    const bool some = in && (l > 0.f || l != l);
-    const float inv = some ? 1.f / l : 0.f;
-    E* orow = static_cast<E*>(a.out) + b * a.so.b + qi * a.so.t + h * a.so.h;
+    __syncthreads();
+    const long parts = static_cast<long>(gridDim.x) * rows;
+    for (int idx = threadIdx.x; idx < rows * kPieces; idx += 256) {
+        const int row = idx / kPieces, piece = idx % kPieces, col = 4 * piece;
+        float mw[4], top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, mw[w] = ml[w * 64 + row]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        f32x4 v = {0};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            typename T::x4 v;
+        for (int w = 0; w < 4; ++w) {
+            const float f = exp2_fast((mw[w] - ref) * sc2);
+            sum = fmaf(ml[w * 64 + 32 + row], f, sum);
+            const f32x4 part = *reinterpret_cast<const f32x4*>(
+                smem + w * 2 * T::kBytes + (row * kPieces + (piece ^ (row & (kPieces - 1)))) * 16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(some ? o[i][4 * g + e] * inv : 0.f);
-            const int c = 32 * i + 8 * g + 4 * hh;
-            if (c < a.D) *reinterpret_cast<typename T::x4*>(orow + c) = v;
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], f, v[e]);
         }
-    if (hh == 0)
-        a.lse[(static_cast<long>(b) * a.H + h) * a.Tq + qi] =
-            some ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+        if (me.count > 1) {
+            const long part = static_cast<long>(blockIdx.x) * rows + row;
+            *reinterpret_cast<f32x4*>(a.parts + part * DP + col) = v;
+            if (piece == 0) *reinterpret_cast<f32x2*>(a.parts + parts * DP + 2 * part) = f32x2{top, sum};
+            continue;
+        }
+        const int qr = row / group, head = hk * group + row % group;
+        const bool some = qr < sq.m && (sum > 0.f || sum != sum);
+        const float inv = some ? 1.f / sum : 0.f;
+        if (col < a.D) {
+            typename T::x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = static_cast<E>(some ? v[e] * inv : 0.f);
+            *reinterpret_cast<typename T::x4*>(static_cast<E*>(a.out) + b * a.so.b + qr * a.so.t + head * a.so.h + col) = y;
+        }
+        if (piece == 0)
+            a.lse[(static_cast<long>(b) * a.H + head) * a.Tq + qr] =
+                some ? top * a.scale + kLn2 * __builtin_amdgcn_logf(sum) : -INFINITY;
+    }
 }
 
 // One wave per row of a sequence that was cut: the chunks' maxima and sums, 64 at a time, then
@@ -670,33 +667,39 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
     const int live = qi < sq.m ? count : 0;
     const long parts = static_cast<long>(workgroups) * rows;
     const float sc2 = a.scale * kLog2e;
-    const float* ml = a.parts + parts * DP;
-    float m = -INFINITY;
-    for (int c = lane; c < live; c += 64) m = fmaxf(m, ml[2 * (static_cast<long>(first + c * a.Hk) * rows + r)]);
+    const f32x2* ml = reinterpret_cast<const f32x2*>(a.parts + parts * DP);
+    constexpr int kFlight = 8;  // parts in flight
+    float v0[kFlight], v1[kFlight];
+    auto pair = [&](int c) {
+        return c < live ? ml[static_cast<long>(first + c * a.Hk) * rows + r] : f32x2{-INFINITY, 0.f};
+    };
+    auto load = [&](int c) {
+        const float* o = a.parts + (static_cast<long>(first) * rows + r) * DP + lane;
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+            const float* oc = o + static_cast<long>(min(c + u, live - 1)) * a.Hk * rows * DP;
+            v0[u] = oc[0];
+            if (DP > 64) v1[u] = oc[64];
+        }
+    };
+    f32x2 mine = pair(lane);
+    if (live > 0) load(0);  // beside the maxima
+    float m = mine[0];
+    for (int c = lane + 64; c < live; c += 64) m = fmaxf(m, pair(c)[0]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     const float ref = m == -INFINITY ? 0.f : m;
     float l = 0.f, o0 = 0.f, o1 = 0.f;
     for (int c0 = 0; c0 < live; c0 += 64) {
-        float w = 0.f;
-        if (c0 + lane < live) {
-            const long p = static_cast<long>(first + (c0 + lane) * a.Hk) * rows + r;
-            w = exp2_fast((ml[2 * p] - ref) * sc2);
-            l = fmaf(ml[2 * p + 1], w, l);
-        }
+        if (c0 > 0) mine = pair(c0 + lane);
+        const float w = exp2_fast((mine[0] - ref) * sc2);
+        l = fmaf(mine[1], w, l);
         const int more = min(64, live - c0);
-        const float* o = a.parts + (static_cast<long>(first + c0 * a.Hk) * rows + r) * DP;
-        for (int c1 = 0; c1 < more; c1 += 8) {  // eight parts in flight
-            float v0[8], v1[8];
+        for (int c1 = 0; c1 < more; c1 += kFlight) {
+            if (c0 + c1 > 0) load(c0 + c1);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float* oc = o + min(c1 + u, more - 1) * static_cast<long>(a.Hk * rows) * DP;
-                v0[u] = oc[lane];
-                if (DP > 64) v1[u] = oc[64 + lane];
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(c1 + u, 63)));
+            for (int u = 0; u < kFlight; ++u) {
+                const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), c1 + u));
                 if (c1 + u < more) {
                     o0 = fmaf(v0[u], wc, o0);
                     if (DP > 64) o1 = fmaf(v1[u], wc, o1);
@@ -1101,11 +1104,6 @@ int launch_fwd(const AttnArgs& a, hipStream_t s) {
 
 // Workgroups that attn_few_kernel cuts the keys for (0: one per sequence and key head; -1: not the
 // few-query form).
-#ifndef FEWWG
-#define FEWWG 512
-#endif
-constexpr int kFewTarget = FEWWG;
-
 int few_target(const AttnArgs& a) {
     if (a.limit != 0 || static_cast<long>(a.Tq) * (a.H / a.Hk) > kFew) return -1;
     return a.B <= kFewMaxBatch && a.B * a.Hk < kFewTarget && a.Tk > 128 ? kFewTarget : 0;
@@ -1115,7 +1113,7 @@ int padded_dim(int D) { return D <= 64 ? 64 : 128; }
 
 template <class E, int DP>
 int launch_few(const AttnArgs& a, hipStream_t s) {
-    constexpr int park = 2 * 64 * (DP / 32 * 16 + 2) * 4, kv = 8 * Tile<E, DP, 32>::kBytes, lds = park > kv ? park : kv;
+    constexpr int lds = 8 * Tile<E, DP, 32>::kBytes + 4 * 64 * 4;
     if (a.target != 0 && a.parts == nullptr) return -2;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_few_kernel<E, DP>), lds)) return st;
     hipLaunchKernelGGL((attn_few_kernel<E, DP>), dim3(few_workgroups(a)), dim3(256), lds, s, a);

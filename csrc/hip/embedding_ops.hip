@@ -56,44 +56,39 @@ __device__ __forceinline__ unsigned key_of(const long* tokens, long i, unsigned 
 }
 
 // Few tokens, one launch: the place of row i is the number of rows with a smaller key, or the
-// same key and a smaller index.  A workgroup holds all keys in LDS and places 64 rows, its 16
-// waves each count one sixteenth of the keys, four per (broadcast) LDS read and two vector
-// instructions each.
+// same key and a smaller index.  A workgroup holds all keys in LDS and places 16 rows: lane l has
+// row l % 16 and looks at every fourth block of 16 keys of its wave, four per LDS read and two vector
+// instructions each.  (Bound by these; 4000 rows: 5.2 us, with 64 rows per workgroup, a quarter as
+// many of them, 10.2.)
 constexpr int kRankWaves = 16, kRankRows = 8192;
 
 __global__ void __launch_bounds__(64 * kRankWaves) rank_kernel(const long* tokens, unsigned V, long padding,
                                                                unsigned* key, unsigned* order, int R) {
     __shared__ __attribute__((aligned(16))) unsigned keys[kRankRows];
-    __shared__ unsigned count[kRankWaves][64];
+    __shared__ unsigned count[kRankWaves][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i0 = blockIdx.x * 64, i = i0 + lane, padded = (R + 63) & ~63;
+    const int row = lane & 15, i0 = blockIdx.x * 16, i = i0 + row, padded = (R + 63) & ~63;
     // (behind the last row: keys that no row is behind)
+#pragma unroll 8
     for (int j = threadIdx.x; j < padded; j += 64 * kRankWaves)
         keys[j] = j < R ? key_of(tokens, j, V, padding) : 0xFFFFFFFFu;
     __syncthreads();
     const unsigned mine = keys[i];  // (i < padded)
-    // 64 keys at a time; equal ones count where their row comes first
-    unsigned n = 0;
-    for (int j0 = wave * 64; j0 < padded; j0 += 64 * kRankWaves) {
-        if (j0 == i0) {
-            for (int j = 0; j < 64; ++j) {
-                const unsigned k = keys[j0 + j];
-                n += k < mine || (k == mine && j < lane);
-            }
-            continue;
-        }
-        const unsigned limit = j0 < i0 ? mine : mine - 1;  // count keys <= limit
-        const bool none = j0 > i0 && mine == 0;
+    // equal keys count in the blocks before the row's own, and in that (a key per wave) before the row
+    unsigned n = lane < 16 && wave < row && keys[i0 + wave] == mine;
+    for (int j0 = wave * 64 + (lane & 48); j0 < padded; j0 += 64 * kRankWaves) {
+        const unsigned limit = mine + (j0 < i0);  // count keys < limit (mine <= V < 2^31)
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) {
+        for (int j = 0; j < 16; j += 4) {
             const uint4 k = *reinterpret_cast<const uint4*>(&keys[j0 + j]);
-            n += (k.x <= limit) + (k.y <= limit) + (k.z <= limit) + (k.w <= limit);
+            n += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
         }
-        if (none) n -= 64;  // (mine - 1 wrapped: every key counted)
     }
-    count[wave][lane] = n;
+    n += __shfl_xor(n, 16, 64);
+    n += __shfl_xor(n, 32, 64);
+    if (lane < 16) count[wave][lane] = n;
     __syncthreads();
-    if (wave != 0 || i >= R) return;
+    if (threadIdx.x >= 16 || i >= R) return;
     unsigned place = 0;
 #pragma unroll
     for (int w = 0; w < kRankWaves; ++w) place += count[w][lane];
@@ -101,29 +96,32 @@ __global__ void __launch_bounds__(64 * kRankWaves) rank_kernel(const long* token
     order[place] = static_cast<unsigned>(i);
 }
 
-// Many tokens: stable counting sort by 8 bits at a time, lowest first, in two launches each: the
-// digits of every tile are counted, then every workgroup finds its own first places from all
-// counts and moves its tile.  A tile is 256 * rounds keys, four waves with 64 * rounds consecutive
-// ones each; with at most 128 tiles the counts are 128 rows of 1 KiB that every workgroup can
-// read for itself, which is cheaper than a launch for their running sums.
-constexpr int kDigits = 256, kMaxTiles = 128;
+// Many tokens: stable counting sort by 8 bits at a time, lowest first.  One launch counts the
+// lowest digits of every tile; then one launch for each digit, in which every workgroup finds its
+// own first places from all counts, moves its tile and counts the next digit of what it moved in
+// the tiles where that lands (whole numbers, so the order of these atomics changes nothing).  A tile
+// is 256 * rounds keys, four waves with 64 * rounds consecutive ones each; with at most 128 tiles
+// the counts are 128 rows of 1 KiB that every workgroup can read for itself, which is cheaper than
+// a launch for their running sums.
+constexpr int kDigits = 256, kMaxTiles = 128, kMaxPasses = 4;
 
 __device__ __forceinline__ unsigned tile_key(const long* tokens, const unsigned* from, long i, unsigned V,
                                              long padding) {
     return tokens != nullptr ? key_of(tokens, i, V, padding) : from[i];
 }
 
-// count[tile][digit]
-__global__ void __launch_bounds__(256) digit_count_kernel(const long* tokens, const unsigned* from,
-                                                          unsigned V, long padding, unsigned* count,
-                                                          long R, int rounds, int shift) {
+// count[tile][digit] of the lowest digit; the counts of `later` digits are set to 0.
+__global__ void __launch_bounds__(256) digit_count_kernel(const long* tokens, unsigned V, long padding,
+                                                          unsigned* count, long R, int rounds, int later) {
     __shared__ unsigned hist[kDigits];
     hist[threadIdx.x] = 0;
+    for (int p = 1; p <= later; ++p) count[(p * kMaxTiles + blockIdx.x) * kDigits + threadIdx.x] = 0;
     __syncthreads();
     const long i0 = static_cast<long>(blockIdx.x) * rounds * 256;
+#pragma unroll 4
     for (int k = 0; k < rounds; ++k) {
         const long i = i0 + k * 256 + threadIdx.x;
-        if (i < R) atomicAdd(&hist[(tile_key(tokens, from, i, V, padding) >> shift) & 255u], 1u);
+        if (i < R) atomicAdd(&hist[key_of(tokens, i, V, padding) & 255u], 1u);
     }
     __syncthreads();
     count[blockIdx.x * kDigits + threadIdx.x] = hist[threadIdx.x];
@@ -134,8 +132,8 @@ __global__ void __launch_bounds__(256) digit_count_kernel(const long* tokens, co
 __global__ void __launch_bounds__(256) digit_move_kernel(const long* tokens, const unsigned* from,
                                                          const unsigned* from_order, unsigned V,
                                                          long padding, const unsigned* count,
-                                                         unsigned* key, unsigned* order, long R,
-                                                         int rounds, int shift) {
+                                                         unsigned* next_count, unsigned* key,
+                                                         unsigned* order, long R, int rounds, int shift) {
     __shared__ unsigned next[4][kDigits];
     __shared__ unsigned sums[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -150,11 +148,15 @@ __global__ void __launch_bounds__(256) digit_move_kernel(const long* tokens, con
     // thread d: keys with digit d in the tiles before this one, and in all
     unsigned before = 0, all = 0;
     const int tiles = gridDim.x, mine = blockIdx.x;
-#pragma unroll 8
-    for (int t = 0; t < tiles; ++t) {
-        const unsigned n = count[t * kDigits + threadIdx.x];
-        before += t < mine ? n : 0u;
-        all += n;
+    for (int t0 = 0; t0 < tiles; t0 += 32) {
+        unsigned n[32];  // (all in flight: the loop's time is that of its loads one after another)
+#pragma unroll
+        for (int t = 0; t < 32; ++t) n[t] = count[min(t0 + t, tiles - 1) * kDigits + threadIdx.x];
+#pragma unroll
+        for (int t = 0; t < 32; ++t) {
+            before += t0 + t < mine ? n[t] : 0u;
+            all += t0 + t < tiles ? n[t] : 0u;
+        }
     }
     unsigned x = all;  // running sum over the digits
 #pragma unroll
@@ -177,6 +179,7 @@ __global__ void __launch_bounds__(256) digit_move_kernel(const long* tokens, con
         const long i = i0 + r * 64 + lane;
         const bool in = i < R;
         const unsigned k = in ? tile_key(tokens, from, i, V, padding) : 0u, d = (k >> shift) & 255u;
+        const unsigned o = in && from_order != nullptr ? from_order[i] : static_cast<unsigned>(i);
         unsigned long same = __ballot(in);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
@@ -193,7 +196,9 @@ __global__ void __launch_bounds__(256) digit_move_kernel(const long* tokens, con
         if (in) {
             const unsigned place = first + static_cast<unsigned>(__popcll(below));
             key[place] = k;
-            order[place] = from_order != nullptr ? from_order[i] : static_cast<unsigned>(i);
+            order[place] = o;
+            if (next_count != nullptr)
+                atomicAdd(&next_count[place / (256u * rounds) * kDigits + ((k >> shift >> 8) & 255u)], 1u);
         }
     }
 }
@@ -350,13 +355,20 @@ __global__ void __launch_bounds__(512) embedding_join_kernel(BwdArgs a) {
     const int ch = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
     const int p0 = ch * a.chunk, pe = p0 + a.chunk;  // (the last chunk has no join)
     if (pe >= a.R) return;
-    const unsigned k = a.key[pe];
-    if (a.key[pe - 1] != k || k >= static_cast<unsigned>(a.V)) return;
-    if (a.key[p0] == k && p0 > 0 && a.key[p0 - 1] == k) return;  // it began before the chunk
+    // the keys at the chunk's borders and at the starts of those behind it, read together
+    const int at = lane == 0 ? p0 - 1 : lane == 1 ? p0 : lane == 2 ? pe - 1 : pe;
+    const unsigned edge = a.key[max(at, 0)];
+    auto start = [&](int c) { return c < a.chunks ? a.key[static_cast<long>(c) * a.chunk] : 0xFFFFFFFFu; };
+    unsigned first = start(ch + 1 + lane);
+    const unsigned k = __builtin_amdgcn_readlane(edge, 3);
+    if (__builtin_amdgcn_readlane(edge, 2) != k || k >= static_cast<unsigned>(a.V)) return;
+    if (p0 > 0 && __builtin_amdgcn_readlane(edge, 1) == k && __builtin_amdgcn_readlane(edge, 0) == k)
+        return;  // it began before the chunk
     // chunks behind this one whose first key is k hold a part in head[]
     int more = 0;
     for (int c0 = ch + 1;; c0 += 64) {
-        const unsigned long same = __ballot(c0 + lane < a.chunks && a.key[static_cast<long>(c0 + lane) * a.chunk] == k);
+        if (c0 > ch + 1) first = start(c0 + lane);
+        const unsigned long same = __ballot(first == k);
         more += __popcll(same);
         if (same != ~0UL) break;
     }
@@ -449,7 +461,7 @@ int nf_embedding_fwd(const long* tokens, const void* table, const void* pos, voi
 
 // unsigned words of scratch that nf_token_order needs
 long nf_token_order_words(long R) {
-    return R <= kRankRows ? 0 : 2 * R + kMaxTiles * kDigits;
+    return R <= kRankRows ? 0 : 2 * R + kMaxPasses * kMaxTiles * kDigits;
 }
 
 // key[i]: the i-th smallest token (V: none, or the padding token), order[i]: its row; equal
@@ -459,7 +471,7 @@ int nf_token_order(const long* tokens, unsigned* key, unsigned* order, unsigned*
     if (R <= 0 || R >= (1L << 31) || V <= 0 || V >= (1L << 31)) return -1;
     const unsigned v = static_cast<unsigned>(V);
     if (R <= kRankRows) {
-        hipLaunchKernelGGL(rank_kernel, dim3(static_cast<unsigned>((R + 63) / 64)), dim3(64 * kRankWaves), 0, s,
+        hipLaunchKernelGGL(rank_kernel, dim3(static_cast<unsigned>((R + 15) / 16)), dim3(64 * kRankWaves), 0, s,
                            tokens, v, padding, key, order, static_cast<int>(R));
         return static_cast<int>(hipGetLastError());
     }
@@ -467,15 +479,16 @@ int nf_token_order(const long* tokens, unsigned* key, unsigned* order, unsigned*
     const dim3 grid(static_cast<unsigned>((R + rounds * 256L - 1) / (rounds * 256L)));
     unsigned *other_key = scratch, *other_order = scratch + R, *count = scratch + 2 * R;
     int passes = 1;
-    while (passes < 4 && (v >> (8 * passes)) != 0) ++passes;
+    while (passes < kMaxPasses && (v >> (8 * passes)) != 0) ++passes;
     const unsigned *from = nullptr, *from_order = nullptr;
+    hipLaunchKernelGGL(digit_count_kernel, grid, dim3(256), 0, s, tokens, v, padding, count, R, rounds, passes - 1);
     for (int p = 0; p < passes; ++p) {
         const bool last = (passes - p) & 1;  // the passes alternate, the last one ends in key / order
         unsigned *to = last ? key : other_key, *to_order = last ? order : other_order;
         const long* tok = p == 0 ? tokens : nullptr;
-        hipLaunchKernelGGL(digit_count_kernel, grid, dim3(256), 0, s, tok, from, v, padding, count, R, rounds, 8 * p);
-        hipLaunchKernelGGL(digit_move_kernel, grid, dim3(256), 0, s, tok, from, from_order, v, padding, count, to,
-                           to_order, R, rounds, 8 * p);
+        unsigned* now = count + p * kMaxTiles * kDigits;
+        hipLaunchKernelGGL(digit_move_kernel, grid, dim3(256), 0, s, tok, from, from_order, v, padding, now,
+                           p + 1 < passes ? now + kMaxTiles * kDigits : nullptr, to, to_order, R, rounds, 8 * p);
         from = to;
         from_order = to_order;
     }

@@ -71,19 +71,31 @@ int launch(const void* x, const void* res, void* y, long R, long C, long ldx, lo
 
 extern "C" {
 
-// type: 0 float, 1 bf16, 2 half.  Rows of C columns, ld elements apart; y may be x or the
+// One argument block instead of fifteen arguments, whose conversion costs the caller more than the
+// launch.  type: 0 float, 1 bf16, 2 half.  Rows of C columns, ld elements apart; y may be x or the
 // residual (with the same distance between rows).  step_at: the step number in device memory,
 // or null for `step`.  first: flattened index of the first element.
-int nf_dropout(const void* x, const void* res, void* y, int type, long R, long C, long ldx, long ldr,
-               long ldy, unsigned limit, unsigned long long seed, const long* step_at, unsigned step,
-               long first, hipStream_t s) {
-    if (R <= 0 || C <= 0 || limit > 65535u || first < 0) return -1;
-    if (R > 1 && (ldx < C || ldy < C || (res != nullptr && ldr < C))) return -2;
-    const DropRows d = {seed, step_at, step, limit, 65536.f / static_cast<float>(65536u - limit), first};
-    switch (type) {
-    case 0: return launch<float>(x, res, y, R, C, ldx, ldr, ldy, d, s);
-    case 1: return launch<bf16>(x, res, y, R, C, ldx, ldr, ldy, d, s);
-    case 2: return launch<half>(x, res, y, R, C, ldx, ldr, ldy, d, s);
+struct DropoutArgs {
+    const void *x, *res;
+    void* y;
+    const long* step_at;
+    long R, C, ldx, ldr, ldy, first;
+    unsigned long long seed;
+    unsigned limit, step;
+    int type, unused;
+};
+
+int nf_dropout_args_size() { return static_cast<int>(sizeof(DropoutArgs)); }
+
+int nf_dropout(const DropoutArgs* args, hipStream_t s) {
+    const DropoutArgs& a = *args;
+    if (a.R <= 0 || a.C <= 0 || a.limit > 65535u || a.first < 0) return -1;
+    if (a.R > 1 && (a.ldx < a.C || a.ldy < a.C || (a.res != nullptr && a.ldr < a.C))) return -2;
+    const DropRows d = {a.seed, a.step_at, a.step, a.limit, 65536.f / static_cast<float>(65536u - a.limit), a.first};
+    switch (a.type) {
+    case 0: return launch<float>(a.x, a.res, a.y, a.R, a.C, a.ldx, a.ldr, a.ldy, d, s);
+    case 1: return launch<bf16>(a.x, a.res, a.y, a.R, a.C, a.ldx, a.ldr, a.ldy, d, s);
+    case 2: return launch<half>(a.x, a.res, a.y, a.R, a.C, a.ldx, a.ldr, a.ldy, d, s);
     default: return -1;
     }
 }

@@ -443,18 +443,38 @@ int bwd(BwdArgs a, hipStream_t s) {
 
 extern "C" {
 
-// tokens: R ids; table [V][C]; pos (may be null): [>= T][C], row r takes position r mod T.
-// type: 0 float, 1 bf16, 2 half (table, pos and out).
-int nf_embedding_fwd(const long* tokens, const void* table, const void* pos, void* out, int type,
-                     long R, long T, long V, long C, float scale, unsigned limit,
-                     unsigned long long seed, const long* step_at, unsigned step, long first,
-                     hipStream_t s) {
-    if (R <= 0 || T <= 0 || V <= 0 || C <= 0 || limit > 65535u || first < 0) return -1;
-    const DropRows d = drop_rows(limit, seed, step_at, step, first);
-    switch (type) {
-    case 0: return fwd<float>(tokens, table, pos, out, R, T, V, C, scale, d, s);
-    case 1: return fwd<bf16>(tokens, table, pos, out, R, T, V, C, scale, d, s);
-    case 2: return fwd<half>(tokens, table, pos, out, R, T, V, C, scale, d, s);
+// The arguments of a call as one block.
+// Forward: table [V][C]; pos (may be null): [>= T][C]; out [B][T][C]; type: 0 float, 1 bf16, 2 half
+// (of all three).
+// Backward: key / order: from nf_token_order, or both null: made here from the tokens.  dx: B T rows
+// of C.  dw [V][C]: written everywhere, or (accumulate) added to where tokens are.  dp (may be null):
+// rows 0 .. T - 1 are written.  type: of dx; grad_type: of dw and dp (0, or the type of dx).
+struct EmbeddingArgs {
+    const long* tokens;
+    union { const void* table; const void* dx; };
+    union { const void* pos; void* dp; };
+    union { void* out; void* dw; };
+    const unsigned *key, *order;
+    float* scratch;
+    const long* step_at;
+    long padding, B, T, V, C, first;
+    unsigned long long seed;
+    double scale;
+    unsigned limit, step;
+    int type, grad_type, accumulate, unused;
+};
+
+int nf_embedding_args_size() { return static_cast<int>(sizeof(EmbeddingArgs)); }
+
+int nf_embedding_fwd(const EmbeddingArgs* args, hipStream_t s) {
+    const EmbeddingArgs& a = *args;
+    if (a.B <= 0 || a.T <= 0 || a.V <= 0 || a.C <= 0 || a.limit > 65535u || a.first < 0) return -1;
+    const DropRows d = drop_rows(a.limit, a.seed, a.step_at, a.step, a.first);
+    const float scale = static_cast<float>(a.scale);
+    switch (a.type) {
+    case 0: return fwd<float>(a.tokens, a.table, a.pos, a.out, a.B * a.T, a.T, a.V, a.C, scale, d, s);
+    case 1: return fwd<bf16>(a.tokens, a.table, a.pos, a.out, a.B * a.T, a.T, a.V, a.C, scale, d, s);
+    case 2: return fwd<half>(a.tokens, a.table, a.pos, a.out, a.B * a.T, a.T, a.V, a.C, scale, d, s);
     default: return -1;
     }
 }
@@ -501,39 +521,35 @@ long nf_embedding_bwd_words(long R, long C, int ordered) {
     return 2 * ((R + chunk - 1) / chunk) * C + (ordered ? 0 : 2 * R + nf_token_order_words(R));
 }
 
-// key / order: from nf_token_order, or both null: made here from the tokens.  dx: B T rows of C.  dw [V][C]: written everywhere, or
-// (accumulate) added to where tokens are.  dp (may be null): rows 0 .. T - 1 are written.
-// type: of dx; grad_type: of dw and dp (0, or the type of dx).
-int nf_embedding_bwd(const long* tokens, const unsigned* key, const unsigned* order, long padding,
-                     const void* dx, void* dw, void* dp, float* scratch, int type, int grad_type, long B, long T, long V, long C, float scale,
-                     int accumulate, unsigned limit, unsigned long long seed, const long* step_at,
-                     unsigned step, long first, hipStream_t s) {
-    if (B <= 0 || T <= 0 || V <= 0 || C <= 0 || limit > 65535u || first < 0) return -1;
+int nf_embedding_bwd(const EmbeddingArgs* args, hipStream_t s) {
+    const EmbeddingArgs& in = *args;
+    const long B = in.B, T = in.T, V = in.V, C = in.C;
+    if (B <= 0 || T <= 0 || V <= 0 || C <= 0 || in.limit > 65535u || in.first < 0) return -1;
     if (V >= (1L << 31) || C >= (1L << 25) || B >= (1L << 31) || T >= (1L << 31) || B * T >= (1L << 31)) return -3;
-    if (grad_type != 0 && grad_type != type) return -1;
+    if (in.grad_type != 0 && in.grad_type != in.type) return -1;
     BwdArgs a = {};
-    a.dx = dx; a.dw = dw; a.dp = dp;
+    a.dx = in.dx; a.dw = in.dw; a.dp = in.dp;
     a.B = B; a.T = T; a.V = V; a.C = C;
     a.R = static_cast<int>(B * T);
     a.slabs = static_cast<int>((C + 511) / 512);
     a.chunk = chunk_of(a.R, a.slabs);
     a.chunks = static_cast<int>((a.R + static_cast<long>(a.chunk) - 1) / a.chunk);
-    a.head = scratch;
-    a.tail = scratch + static_cast<long>(a.chunks) * C;
-    a.accumulate = accumulate;
-    a.scale = scale;
-    a.d = drop_rows(limit, seed, step_at, step, first);
+    a.head = in.scratch;
+    a.tail = in.scratch + static_cast<long>(a.chunks) * C;
+    a.accumulate = in.accumulate;
+    a.scale = static_cast<float>(in.scale);
+    a.d = drop_rows(in.limit, in.seed, in.step_at, in.step, in.first);
     if (static_cast<long>(a.chunks) * a.slabs > (1L << 22)) return -3;
-    if (key == nullptr || order == nullptr) {
-        unsigned* words = reinterpret_cast<unsigned*>(scratch + 2 * static_cast<long>(a.chunks) * C);
-        const int status = nf_token_order(tokens, words, words + a.R, words + 2L * a.R, a.R, V, padding, s);
+    a.key = in.key;
+    a.order = in.order;
+    if (a.key == nullptr || a.order == nullptr) {
+        unsigned* words = reinterpret_cast<unsigned*>(in.scratch + 2 * static_cast<long>(a.chunks) * C);
+        const int status = nf_token_order(in.tokens, words, words + a.R, words + 2L * a.R, a.R, V, in.padding, s);
         if (status != 0) return status;
-        key = words;
-        order = words + a.R;
+        a.key = words;
+        a.order = words + a.R;
     }
-    a.key = key;
-    a.order = order;
-    switch (type * 4 + grad_type) {
+    switch (in.type * 4 + in.grad_type) {
     case 0: return bwd<float, float>(a, s);
     case 4: return bwd<bf16, float>(a, s);
     case 5: return bwd<bf16, bf16>(a, s);

@@ -257,9 +257,9 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     the Philox4x32-7 block with counter ``(j >> 2, i >> 2, (first_batch + b) H + h, step)``."""
     a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if lse is None:
-        lse = torch.empty(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device)
+        lse = q.new_empty((a.B, a.H, a.Tq), dtype=torch.float32)
     to = _operand(out, "out", q.shape, q, True)
     _check_lse(lse, a, q)
     if a.B == 0 or a.Tq == 0:
@@ -280,7 +280,7 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
         if floats:
             # (scratch of its own for every call: the allocator hands it on in stream order, and a
             # captured call's belongs to its graph)
-            parts = torch.empty(floats, dtype=torch.float32, device=dev)
+            parts = q.new_empty(floats, dtype=torch.float32)
             packed = a.pack(lse.data_ptr(), to, parts=parts.data_ptr())
         library.check(_fn("nf_attention")(packed, _TYPES[q.dtype], 0, library.stream_ptr(dev)), "attention_fwd")
     return out, lse
@@ -322,7 +322,7 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     dev = q.device
     with library.on_device(dev):
         floats = _fn("nf_attention_bwd_floats")(a.pack(0, _NONE))
-        scratch = torch.empty(floats, dtype=torch.float32, device=dev)
+        scratch = q.new_empty(floats, dtype=torch.float32)
         library.check(_fn("nf_attention")(a.pack(lse.data_ptr(), *operands, delta=scratch.data_ptr()),
                                           _TYPES[q.dtype], 1, library.stream_ptr(dev)), "attention_bwd")
 

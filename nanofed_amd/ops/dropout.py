@@ -16,7 +16,8 @@ also what the kernel tests compare against.  The reference applies ``F.dropout``
 from __future__ import annotations
 
 import hashlib
-from ctypes import c_int, c_long, c_uint, c_ulonglong, c_void_p
+import struct
+from ctypes import c_char_p, c_int, c_void_p
 
 import torch
 
@@ -24,8 +25,11 @@ from nanofed_amd.core.exceptions import DeviceError
 
 from . import library
 
-P, L, I, U, UL = c_void_p, c_long, c_int, c_uint, c_ulonglong
-_SIGS = {"nf_dropout": ([P, P, P, I, L, L, L, L, L, U, UL, P, U, L, P], I)}
+_SIGS = {
+    "nf_dropout_args_size": ([], c_int),
+    "nf_dropout": ([c_char_p, c_void_p], c_int),
+}
+_ARGS = struct.Struct("@4P6qQ2I2i")  # DropoutArgs of csrc/hip/dropout_ops.hip
 _fns: dict[str, object] = {}
 
 FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -71,11 +75,16 @@ def check_key(seed: int, step: "int | torch.Tensor", device: torch.device, what:
         raise DeviceError(f"{what}: the step must be a 32-bit unsigned number")
 
 
-def step_args(step: "int | torch.Tensor") -> tuple[int | None, int]:
-    """(address of the step in device memory, its value when it is a plain number)."""
+def step_args(step: "int | torch.Tensor") -> tuple[int, int]:
+    """(address of the step in device memory or 0, its value when it is a plain number)."""
     if isinstance(step, torch.Tensor):
         return step.data_ptr(), 0
-    return None, step
+    return 0, step
+
+
+def check_first(first: int, what: str) -> None:
+    if not 0 <= first < 1 << 62:
+        raise DeviceError(f"{what}: first must not be negative (nor pass 2^62)")
 
 
 def philox_words(seed: int, step: "int | torch.Tensor", c0: torch.Tensor, c1: torch.Tensor,
@@ -118,11 +127,10 @@ def dropout_fwd(x: torch.Tensor, p: float, *, seed: int, step: "int | torch.Tens
     limit = limit_of(p, 16, "dropout")
     if x.dtype not in FLOAT_TYPES:
         raise DeviceError(f"dropout: float32, bfloat16 or float16, got {x.dtype}")
-    if first < 0:
-        raise DeviceError("dropout: first must not be negative")
+    check_first(first, "dropout")
     check_key(seed, step, x.device, "dropout")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     for t, name in ((residual, "residual"), (out, "out")):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
             raise DeviceError(f"dropout: {name} must have the shape, type and device of x")
@@ -144,10 +152,11 @@ def dropout_fwd(x: torch.Tensor, p: float, *, seed: int, step: "int | torch.Tens
         (R, C), ld, ldo = x.shape, x.stride(0), out.stride(0)
         ldr = residual.stride(0) if residual is not None else 0
     at, number = step_args(step)
-    with library.on_device(x.device):
-        library.check(_fn("nf_dropout")(
-            x.data_ptr(), residual.data_ptr() if residual is not None else None, out.data_ptr(),
-            FLOAT_TYPES[x.dtype], R, C, ld, ldr, ldo, limit, seed, at, number, first, library.stream_ptr(x.device)), "dropout")
+    args = _ARGS.pack(x.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(), at,
+                      R, C, ld, ldr, ldo, first, seed, limit, number, FLOAT_TYPES[x.dtype], 0)
+    dev = x.device
+    with library.on_device(dev):
+        library.check(_fn("nf_dropout")(args, library.stream_ptr(dev)), "dropout")
     return out
 
 

@@ -15,23 +15,27 @@ reference has no sequence model; this serves the GPT-2 configuration of the benc
 
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_long, c_uint, c_ulonglong, c_void_p
+import struct
+from ctypes import c_char_p, c_int, c_long, c_void_p
+from functools import lru_cache
 
 import torch
 
 from nanofed_amd.core.exceptions import DeviceError
 
 from . import library
-from .dropout import FLOAT_TYPES, check_key, kept_rows, limit_of, step_args
+from .dropout import FLOAT_TYPES, check_first, check_key, kept_rows, limit_of, step_args
 
-P, L, I, U, UL, FL = c_void_p, c_long, c_int, c_uint, c_ulonglong, c_float
+P, L, I, ARGS = c_void_p, c_long, c_int, c_char_p
 _SIGS = {
-    "nf_embedding_fwd": ([P, P, P, P, I, L, L, L, L, FL, U, UL, P, U, L, P], I),
+    "nf_embedding_fwd": ([ARGS, P], I),
     "nf_token_order_words": ([L], L),
     "nf_token_order": ([P, P, P, P, L, L, L, P], I),
     "nf_embedding_bwd_words": ([L, L, I], L),
-    "nf_embedding_bwd": ([P, P, P, L, P, P, P, P, I, I, L, L, L, L, FL, I, U, UL, P, U, L, P], I),
+    "nf_embedding_bwd": ([ARGS, P], I),
+    "nf_embedding_args_size": ([], I),
 }
+_ARGS = struct.Struct("@8P6qQd2I4i")  # EmbeddingArgs of csrc/hip/embedding_ops.hip
 _fns: dict[str, object] = {}
 
 
@@ -48,8 +52,13 @@ def symbols() -> list[str]:
     return sorted(_SIGS)
 
 
-def _address(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+def _address(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+@lru_cache(maxsize=256)
+def _bwd_words(rows: int, columns: int, ordered: bool) -> int:
+    return _fn("nf_embedding_bwd_words")(rows, columns, ordered)
 
 
 def _need(t: torch.Tensor, shape: tuple, dtypes, device: torch.device, name: str) -> None:
@@ -80,14 +89,13 @@ def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor |
     B, T = _tokens(tokens, dev)
     limit = limit_of(dropout, 16, "embedding")
     check_key(seed, step, dev, "embedding")
-    if first < 0:
-        raise DeviceError("embedding: first must not be negative")
+    check_first(first, "embedding")
     if positions is not None:
         if positions.dim() != 2 or positions.shape[0] < T:
             raise DeviceError(f"embedding: positions must have at least {T} rows")
         _need(positions, (positions.shape[0], C), (table.dtype,), dev, "positions")
     if out is None:
-        out = torch.empty(*tokens.shape, C, dtype=table.dtype, device=dev)
+        out = table.new_empty((*tokens.shape, C))
     elif out.numel() != B * T * C or out.shape[-1] != C:
         raise DeviceError(f"embedding: out must hold {B * T} rows of {C}")
     else:
@@ -106,10 +114,10 @@ def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor |
         out.copy_(x.view(out.shape))
         return out
     at, number = step_args(step)
+    args = _ARGS.pack(tokens.data_ptr(), table.data_ptr(), _address(positions), out.data_ptr(), 0, 0, 0, at,
+                      -1, B, T, V, C, first, seed, scale, limit, number, FLOAT_TYPES[table.dtype], 0, 0, 0)
     with library.on_device(dev):
-        library.check(_fn("nf_embedding_fwd")(
-            tokens.data_ptr(), table.data_ptr(), _address(positions), out.data_ptr(), FLOAT_TYPES[table.dtype], B * T, T, V, C, scale, limit, seed, at, number,
-            first, library.stream_ptr(dev)), "embedding_fwd")
+        library.check(_fn("nf_embedding_fwd")(args, library.stream_ptr(dev)), "embedding_fwd")
     return out
 
 
@@ -170,8 +178,7 @@ def embedding_bwd(tokens: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor
     padding = _padding(padding_idx, V)
     limit = limit_of(dropout, 16, "embedding")
     check_key(seed, step, dev, "embedding")
-    if first < 0:
-        raise DeviceError("embedding: first must not be negative")
+    check_first(first, "embedding")
     if dout.numel() != R * C or (dout.numel() and dout.shape[-1] != C) or not dout.is_contiguous():
         raise DeviceError(f"embedding: dout must be {R} contiguous rows of {C}")
     _need(dtable, (V, C), (dout.dtype, torch.float32), dev, "dtable")
@@ -209,10 +216,9 @@ def embedding_bwd(tokens: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor
     at, number = step_args(step)
     # (scratch of its own for every call: the allocator hands it on in stream order, and a captured
     # call's belongs to its graph)
-    scratch = torch.empty(_fn("nf_embedding_bwd_words")(R, C, order is not None), dtype=torch.float32, device=dev)
+    scratch = dout.new_empty(_bwd_words(R, C, order is not None), dtype=torch.float32)
+    args = _ARGS.pack(tokens.data_ptr(), dout.data_ptr(), _address(dpositions), dtable.data_ptr(), _address(key),
+                      _address(rows), scratch.data_ptr(), at, padding, B, T, V, C, first, seed, scale, limit, number,
+                      FLOAT_TYPES[dout.dtype], FLOAT_TYPES[dtable.dtype], bool(accumulate), 0)
     with library.on_device(dev):
-        library.check(_fn("nf_embedding_bwd")(
-            tokens.data_ptr(), _address(key), _address(rows), padding, dout.data_ptr(), dtable.data_ptr(),
-            _address(dpositions), scratch.data_ptr(), FLOAT_TYPES[dout.dtype], FLOAT_TYPES[dtable.dtype],
-            B, T, V, C, scale, accumulate, limit, seed, at, number, first, library.stream_ptr(dev)),
-            "embedding_bwd")
+        library.check(_fn("nf_embedding_bwd")(args, library.stream_ptr(dev)), "embedding_bwd")

@@ -98,12 +98,13 @@ def stream_ptr(device: torch.device | None = None) -> c_void_p:
 
 
 _SAME_DEVICE = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device(device: torch.device):
     """Context in which launches go to ``device`` (a kernel is launched on the current device,
     whatever stream it is given); free when that is the current one already."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _current_device():
         return _SAME_DEVICE
     return torch.cuda.device(device)
 

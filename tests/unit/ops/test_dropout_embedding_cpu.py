@@ -9,6 +9,7 @@ import torch
 from nanofed_amd.core.exceptions import DeviceError
 from nanofed_amd.ops import dropout as D
 from nanofed_amd.ops import embedding as E
+from nanofed_amd.ops import library
 from tests import transformer_oracles as oracle
 
 BF = torch.bfloat16
@@ -133,3 +134,20 @@ def test_embedding_refusals():
                        (dict(order=(torch.zeros(6), torch.zeros(6))), "key"), (dict(dropout=math.nan), "in \\[0, 1\\)")]:
         with pytest.raises(DeviceError, match=match):
             E.embedding_bwd(**{"tokens": tok, "dout": dout, "dtable": table, **how})
+
+
+def test_argument_blocks_have_the_kernels_layout():
+    lib = library.hip_lib()
+    assert D._ARGS.size == lib.nf_dropout_args_size()
+    assert E._ARGS.size == lib.nf_embedding_args_size()
+
+
+def test_places_beyond_62_bits_are_refused():
+    x, tokens, table = torch.zeros(8), torch.zeros(2, dtype=torch.int64), torch.zeros(3, 8)
+    for first in (-1, 1 << 62):
+        with pytest.raises(DeviceError, match="first"):
+            D.dropout_fwd(x, 0.5, seed=1, first=first)
+        with pytest.raises(DeviceError, match="first"):
+            E.embedding_fwd(tokens, table, first=first)
+        with pytest.raises(DeviceError, match="first"):
+            E.embedding_bwd(tokens, torch.zeros(2, 8), table, first=first)

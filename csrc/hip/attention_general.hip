@@ -61,9 +61,7 @@ __device__ __forceinline__ halfx4 tr4(const half* p) {
     return __builtin_bit_cast(halfx4, v);
 }
 
-constexpr int kStage = 64;  // keys per LDS stage of the forward kernel
-// keys (or queries) per LDS stage of the backward kernels
-template <int DP> constexpr int kBwdStage = DP == 64 ? 64 : 32;
+constexpr int kStage = 64;  // keys (or queries) per LDS stage
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Strides { long b, t, h; };  // elements between sequences, rows, heads
@@ -85,7 +83,7 @@ struct AttnArgs {
     unsigned limit, step;
     float* parts;             // partial results of key chunks (few queries) or query ranges (dK / dV)
     int target;               // few queries: workgroups to cut the keys for (0: not cut)
-    int splits;               // dK / dV: query ranges
+    int splits;               // dK / dV: query ranges at most
 };
 
 // -- tiles ------------------------------------------------------------------------------------
@@ -277,6 +275,31 @@ __device__ __forceinline__ int keys_seen(const Seq& s, int i) {  // (i + off fit
     return min(s.n, max(0, i + s.off + 1));
 }
 
+// What a tile of 128 keys reads in the dK / dV kernel: per head the stages from the first one with a
+// query that sees a key of it (query i sees key j from i >= j - off on), and the ranges that these
+// stages of all heads are cut into.
+// Stages that a range of the dK / dV kernel has at least (6 ragged sequences of up to 777, 16 heads on
+// 4: 56.7 us with 6 and 62 with 10 at 64 columns, where two workgroups share a CU; 105 and 98 at 128).
+__host__ __device__ constexpr int least_range(int D) { return D > 64 ? 10 : 6; }
+
+struct KeyPlan { int first, per, ranges; };
+
+__device__ __forceinline__ KeyPlan key_plan(const AttnArgs& a, const Seq& s, int tile0) {
+    if (tile0 >= s.n) return {0, 0, 1};
+    const int first = a.causal ? max(0, tile0 - s.off) / kStage : 0;
+    const int per = max(0, (s.m + kStage - 1) / kStage - first);
+    return {first, per, min(a.splits, max(1, (per * (a.H / a.Hk) + least_range(a.D) - 1) / least_range(a.D)))};
+}
+
+// The sequence and head of a workgroup, `heads` of them per sequence.  Workgroups go to the XCDs and to
+// the quarters of each in turn, whatever these have to do: where lengths differ the sequences are
+// shifted by one from tile to tile, or every tile of a sequence would go to the same place.  (The dQ
+// kernel on six lengths of 0 .. 777: 51 .. 63 us by their order, 47 .. 53 shifted.)
+__device__ __forceinline__ int shifted_head(const AttnArgs& a, int heads) {
+    if (a.klen == nullptr && a.qlen == nullptr) return blockIdx.x;
+    return static_cast<int>((blockIdx.x + static_cast<unsigned long>(heads) * blockIdx.y) % gridDim.x);
+}
+
 __device__ __forceinline__ unsigned step_of(const AttnArgs& a) {
     return a.step_at != nullptr ? static_cast<unsigned>(*a.step_at) : a.step;
 }
@@ -292,7 +315,7 @@ attn_fwd_kernel(AttnArgs a) {
     typedef typename T::x8 x8;
     constexpr int NB = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+    const int bh = shifted_head(a, a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const int tile0 = (gridDim.y - 1 - blockIdx.y) * 128;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
@@ -730,11 +753,11 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
 template <class E, int DP, bool kDrop>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dq_kernel(AttnArgs a) {
-    constexpr int R = kBwdStage<DP>, NB = DP / 32;
+    constexpr int R = kStage, NB = DP / 32;
     typedef Tile<E, DP, R> T;
     typedef typename T::x8 x8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+    const int bh = shifted_head(a, a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
     const int tile0 = (gridDim.y - 1 - blockIdx.y) * 128;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
@@ -875,20 +898,23 @@ attn_dq_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Backward, keys: one workgroup = 128 keys of one key head; streams Q / dO of every query head
 // that reads them.  Where that makes too few workgroups (few sequences, shared heads) the stages of
-// all heads are cut into `splits` ranges, one workgroup each (blockIdx.z): they leave fp32 sums in
+// all heads are cut into ranges (key_plan), one workgroup each (blockIdx.z): they leave fp32 sums in
 // `parts` ([range][dK, dV][B][Hk][Tk][DP]) that attn_add_kernel adds in order.  (6 ragged sequences
-// of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 66 + 10 us in four times as many.)
+// of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 57 + 9 us in ranges.)
 template <class E, int DP, bool kDrop>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dkdv_kernel(AttnArgs a) {
-    constexpr int R = kBwdStage<DP>, NB = DP / 32;
+    constexpr int R = kStage, NB = DP / 32;
     typedef Tile<E, DP, R> T;
     typedef typename T::x8 x8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int bh = blockIdx.x, b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
+    const int bh = shifted_head(a, a.Hk), b = bh / a.Hk, hk = bh % a.Hk, group = a.H / a.Hk;
     const int tile0 = blockIdx.y * 128;  // key tile 0 is seen by every query: longest first
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
+    const KeyPlan plan = key_plan(a, sq, tile0);
+    const int z = blockIdx.z, first = plan.first, per = plan.per;
+    if (z >= plan.ranges) return;
     const int key0 = __builtin_amdgcn_readfirstlane(tile0 + wave * 32), kj = key0 + n;
     const typename T::Lane at = T::lane_offsets(lane);
     x8 kf[DP / 16], vf[DP / 16];
@@ -899,16 +925,12 @@ attn_dkdv_kernel(AttnArgs a) {
     for (int i = 0; i < NB; ++i) { dk[i] = f32x16{0}; dv[i] = f32x16{0}; }
     const float sc2 = a.scale * kLog2e;
     const unsigned step = kDrop ? step_of(a) : 0u;
-    // query i sees key j from i >= j - off on
-    const int first = tile0 < sq.n && a.causal ? max(0, tile0 - sq.off) / R : 0;
-    const int stages = tile0 < sq.n ? (sq.m + R - 1) / R : 0;
 
     constexpr int kBuf = 2 * T::kBytes + 2 * R * 4;
     typename T::Regs qr, dr;
     float ls = 0.f, de = 0.f;
-    const int per = max(0, stages - first);
-    const int it0 = static_cast<int>(static_cast<long>(per) * group * blockIdx.z / a.splits);
-    const int it1 = static_cast<int>(static_cast<long>(per) * group * (blockIdx.z + 1) / a.splits);
+    const int it0 = static_cast<int>(static_cast<long>(per) * group * z / plan.ranges);
+    const int it1 = static_cast<int>(static_cast<long>(per) * group * (z + 1) / plan.ranges);
     for (int g = 0; g < group; ++g) {
         const int h = hk * group + g;
         const int lo = first + max(0, it0 - g * per), hi = first + min(per, it1 - g * per);  // stages of this head
@@ -1026,9 +1048,9 @@ attn_dkdv_kernel(AttnArgs a) {
     // register r of block i: key key0 + acc_row(r), column 32 i + n.  (The factor of what is kept
     // comes last: the probabilities are rounded without it, so that a probability of 1 stays exact.)
     const float up = kDrop ? a.up : 1.f;
-    if (a.splits > 1) {
+    if (plan.ranges > 1) {
         const long heads = static_cast<long>(a.B) * a.Hk;
-        float* pk = a.parts + ((2L * blockIdx.z * heads + bh) * a.Tk) * DP;
+        float* pk = a.parts + ((2L * z * heads + bh) * a.Tk) * DP;
         float* pv = pk + heads * a.Tk * DP;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -1070,14 +1092,17 @@ __global__ void __launch_bounds__(256) attn_add_kernel(AttnArgs a) {
     const int c = static_cast<int>(e % DP), j = static_cast<int>(row % a.Tk);
     const int b = static_cast<int>(row / a.Tk / a.Hk), hk = static_cast<int>(row / a.Tk % a.Hk);
     if (c >= a.D) return;
+    const Seq sq = sequence(a, b);
+    const int ranges = key_plan(a, sq, j & ~127).ranges;
+    if (ranges == 1) return;  // written already
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    if (j < sequence(a, b).n) {
+    if (j < sq.n) {
         const float* p = a.parts + at;
-        for (int z0 = 0; z0 < a.splits; z0 += 4) {
+        for (int z0 = 0; z0 < ranges; z0 += 4) {
             f32x4 x[4];
 #pragma unroll
             for (int z = 0; z < 4; ++z)
-                x[z] = z0 + z < a.splits ? *reinterpret_cast<const f32x4*>(p + 2 * one * (z0 + z)) : f32x4{0.f, 0.f, 0.f, 0.f};
+                x[z] = z0 + z < ranges ? *reinterpret_cast<const f32x4*>(p + 2 * one * (z0 + z)) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int z = 0; z < 4; ++z) sum += x[z];
         }
@@ -1123,14 +1148,13 @@ int launch_few(const AttnArgs& a, hipStream_t s) {
     return static_cast<int>(hipGetLastError());
 }
 
-// Query ranges of the dK / dV kernel: about two rounds of workgroups, while a range keeps six
-// stages (the sums of the ranges cost a launch and their way through memory) and there are at most
-// eight.
+// Query ranges of the dK / dV kernel at most: two rounds of workgroups if all sequences were of full
+// length (the sums of the ranges cost a launch and their way through memory), no more than eight.
+// (Three rounds: 814 instead of 717 us with 2 sequences of 4096, 16 heads on 4 of 128.)
 int key_splits(const AttnArgs& a) {
     const long groups = static_cast<long>(a.B) * a.Hk * ((a.Tk + 127) / 128);
-    const int wide = a.D > 64, rows = wide ? kBwdStage<128> : kBwdStage<64>;
-    const long most = static_cast<long>(a.H / a.Hk) * ((a.Tq + rows - 1) / rows) / 6;
-    const long want = ((wide ? 512 : 1024) + groups - 1) / groups;
+    const long most = static_cast<long>(a.H / a.Hk) * ((a.Tq + kStage - 1) / kStage) / least_range(a.D);
+    const long want = ((a.D > 64 ? 512 : 1024) + groups - 1) / groups;
     const long n = want < most ? want : most;
     return static_cast<int>(n < 1 ? 1 : n > 8 ? 8 : n);
 }
@@ -1138,7 +1162,7 @@ long delta_floats(const AttnArgs& a) { return (static_cast<long>(a.B) * a.H * a.
 
 template <class E, int DP, bool kDrop>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {
-    constexpr int rows = kBwdStage<DP>;
+    constexpr int rows = kStage;
     constexpr int lds = 4 * Tile<E, DP, rows>::kBytes, lds2 = lds + 4 * rows * 4;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop>), lds)) return st;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_dkdv_kernel<E, DP, kDrop>), lds2)) return st;

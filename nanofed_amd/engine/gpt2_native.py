@@ -254,8 +254,10 @@ class GPT2NativeTrainer(GroupTrainer):
         return _Masks(self, step, self.shards.client_ids[k]) if self.m.drops() else None
 
     def _step_number(self, round_idx: int, epoch: int, step: int) -> int:
-        per = max(self.shards.max_steps(), 1)
-        return ((round_idx * self.cfg.local_epochs + epoch) * per + step) & 0xFFFFFFFF
+        """The number that a step's masks are drawn with: of (round, epoch, step) only, whatever
+        shards this rank holds.  Multiples of 2^32 over the golden ratio keep the numbers of different
+        epochs more than 2^32 / (3 epochs) steps apart."""
+        return ((round_idx * self.cfg.local_epochs + epoch) * 0x9E3779B1 + step) & 0xFFFFFFFF
 
     def _embed(self, tokens: torch.Tensor, w: dict[str, torch.Tensor], seq: int, out: torch.Tensor,
                masks: _Masks | None, client: int = 0) -> None:

@@ -248,7 +248,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     anything.  With ``causal`` the last query sees every key: key j is seen by query i where
     ``j <= i + keys - queries`` (equal numbers: the usual triangle; one query: all of the cache).
     Queries behind the length and queries that see no key give 0 and a log-sum-exp of -inf.  A
-    non-finite value that some query sees may spread to other queries of its sequence.
+    non-finite value that some query sees may spread to other queries of its sequence.  ``out`` and
+    ``lse`` must not overlap what is read.
 
     ``dropout`` (taken to a multiple of 1 / 256): each probability is dropped with it, what stays is
     scaled by the inverse of the share that stays.  The mask is a function of ``seed``, ``step`` (a

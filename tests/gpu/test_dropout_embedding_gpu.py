@@ -167,6 +167,12 @@ def test_token_order(R, V):
     assert torch.equal(key.cpu(), want_key) and torch.equal(order.cpu(), want_order)
 
 
+@pytest.mark.parametrize("R,V", [(32_768, 1 << 16), (100_001, (1 << 24) + 5), (300_000, 3)])
+def test_token_order_of_many_and_large_tokens(R, V):
+    """Tiles of several rounds, one to four digits."""
+    test_token_order(R, V)
+
+
 def test_embedding_step_in_a_graph():
     B, T, V, C = 4, 600, 500, 128
     tok, table = uniform(B, T, V).to(DEV), rand(V, C, seed=1, dtype=BF).to(DEV)

@@ -92,3 +92,11 @@ def test_a_short_batch_draws_the_first_masks_of_its_clients_own_range():
         tr.loss_and_grads(1, toks[:n], 3)
         kept.append(tr._buffers(n, toks.shape[1] - 1).x[0].clone())
     assert torch.equal(kept[0][: len(kept[1])], kept[1]) and (kept[1] == 0).any()
+
+
+def test_step_numbers_do_not_depend_on_the_shards_of_the_rank():
+    a, b = _engine(local_epochs=2), _engine(local_epochs=2, samples_per_client=10)
+    at = [(r, e, s) for r in range(40) for e in range(2) for s in range(50)]
+    numbers = [a.trainer._step_number(*x) for x in at]
+    assert numbers == [b.trainer._step_number(*x) for x in at]
+    assert len(set(numbers)) == len(at)

@@ -63,6 +63,11 @@ __device__ __forceinline__ halfx4 tr4(const half* p) {
 
 constexpr int kStage = 64;  // keys (or queries) per LDS stage
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// The reference that scores are taken relative to follows the running maximum only where that gets
+// ahead by a factor of 2^8 in the probability: any reference gives the same quotients, up to 2^8 fits
+// every type here with the same relative rounding, and what the sums so far would have to be
+// multiplied by at nearly every tile (some of 32 rows finds a new maximum) is spared.
+constexpr float kSlack = 8.f;
 
 struct Strides { long b, t, h; };  // elements between sequences, rows, heads
 
@@ -366,7 +371,7 @@ attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
         mx = max_halves(mx);
-        if (__any(mx > m)) {  // the running maximum rarely moves after the first tiles
+        if (__any((mx - m) * sc2 > kSlack)) {
             const float mn = fmaxf(m, mx);
             const float ref = mn == -INFINITY ? 0.f : mn;
             const float alpha = exp2_fast((m - ref) * sc2);
@@ -588,7 +593,7 @@ attn_few_kernel(AttnArgs a) {
             mx = fmaxf(mx, s[r]);
         }
         mx = max_halves(mx);
-        if (__any(mx > m)) {
+        if (__any((mx - m) * sc2 > kSlack)) {
             const float mn = fmaxf(m, mx);
             const float ref = mn == -INFINITY ? 0.f : mn;
             const float alpha = exp2_fast((m - ref) * sc2);

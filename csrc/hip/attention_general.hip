@@ -316,19 +316,23 @@ __device__ __forceinline__ unsigned step_of(const AttnArgs& a) {
 // pairs seen; 32 x 1024 x 12 with dropout: 123 us.  Bound by the vector work on the probabilities
 // (an exponential, a maximum, a sum and a rounding each, half as much again with the mask) beside the
 // two products, at the clock that the power limit leaves (1.9 GHz).
-template <class E, int DP, bool kDrop>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 3 : 2)))
+//
+// KG = 2: a workgroup has 64 queries and two waves for each 32 of them, which take the even and the
+// odd tiles of keys and are joined through LDS at the end.  Twice as many workgroups of half the
+// length, for launches that the longest workgroup would hold up (see halve_keys).
+template <class E, int DP, bool kDrop, int KG>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((DP == 64 ? 4 : 3) - KG)))
 attn_fwd_kernel(AttnArgs a) {
     typedef Tile<E, DP, kStage> T;
     typedef typename T::x8 x8;
-    constexpr int NB = DP / 32;
+    constexpr int NB = DP / 32, W = 4 / KG, kQueries = 32 * W;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int bh = shifted_head(a, a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
-    const int tile0 = (gridDim.y - 1 - blockIdx.y) * 128;
+    const int tile0 = (gridDim.y - 1 - blockIdx.y) * kQueries;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
-    const int q0 = tile0 + wave * 32, qi = q0 + n;
-    const int stages = tile0 < sq.m ? (keys_seen(sq, min(tile0 + 127, sq.m - 1)) + kStage - 1) / kStage : 0;
+    const int grp = __builtin_amdgcn_readfirstlane(wave / W), q0 = tile0 + wave % W * 32, qi = q0 + n;
+    const int stages = tile0 < sq.m ? (keys_seen(sq, min(tile0 + kQueries - 1, sq.m - 1)) + kStage - 1) / kStage : 0;
     const typename T::From kfrom = T::from(a.k, b * a.sk.b + hk * a.sk.h, a.sk.t, sq.n, a.D, tid);
     const typename T::From vfrom = T::from(a.v, b * a.sv.b + hk * a.sv.h, a.sv.t, sq.n, a.D, tid);
     const typename T::Lane at = T::lane_offsets(lane);
@@ -344,7 +348,8 @@ attn_fwd_kernel(AttnArgs a) {
     const int seen_hi = __builtin_amdgcn_readfirstlane(q0 < sq.m ? keys_seen(sq, q0 + 31) : 0);
     const unsigned step = kDrop ? step_of(a) : 0u, head = static_cast<unsigned>(a.first_head + bh);
 
-    typename T::Regs kr, vr;
+    typename T::Regs kr[KG], vr[KG];
+    constexpr int kBuf = 2 * KG * T::kBytes;
     auto tile = [&](const char* Ks, const char* Vs, int key0) {
         f32x16 s[2] = {{0}, {0}};
 #pragma unroll
@@ -415,28 +420,58 @@ attn_fwd_kernel(AttnArgs a) {
             }
         }
     };
-    auto stage = [&](int st, char* here, char* there) {
-        if (st + 1 < stages) {
-            kr = T::load(kfrom, st + 1);
-            vr = T::load(vfrom, st + 1);
+    auto fetch = [&](int it) {
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+            kr[g] = T::load(kfrom, it * KG + g);
+            vr[g] = T::load(vfrom, it * KG + g);
         }
-        if (st * kStage < seen_hi) tile(here, here + T::kBytes, st * kStage);  // wave-uniform
-        if (st + 1 < stages) {
-            T::store(there, kr, tid);
-            T::store(there + T::kBytes, vr, tid);
+    };
+    auto put = [&](char* to) {
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+            T::store(to + 2 * g * T::kBytes, kr[g], tid);
+            T::store(to + (2 * g + 1) * T::kBytes, vr[g], tid);
         }
+    };
+    const int turns = (stages + KG - 1) / KG;
+    auto turn = [&](int it, char* here, char* there) {
+        if (it + 1 < turns) fetch(it + 1);
+        const int key0 = (it * KG + grp) * kStage;
+        const char* at0 = here + 2 * grp * T::kBytes;
+        if (key0 < seen_hi) tile(at0, at0 + T::kBytes, key0);  // wave-uniform
+        if (it + 1 < turns) put(there);
         __syncthreads();
     };
-    if (stages > 0) {
-        kr = T::load(kfrom, 0);
-        vr = T::load(vfrom, 0);
-        T::store(smem, kr, tid);
-        T::store(smem + T::kBytes, vr, tid);
+    if (turns > 0) {
+        fetch(0);
+        put(smem);
     }
     __syncthreads();
-    for (int st = 0; st < stages; st += 2) {
-        stage(st, smem, smem + 2 * T::kBytes);
-        if (st + 1 < stages) stage(st + 1, smem + 2 * T::kBytes, smem);
+    for (int it = 0; it < turns; it += 2) {
+        turn(it, smem, smem + kBuf);
+        if (it + 1 < turns) turn(it + 1, smem + kBuf, smem);
+    }
+    if (KG == 2) {
+        float* park = reinterpret_cast<float*>(smem) + (wave % W) * 64 * (NB * 16 + 2) + lane;
+        if (grp == 1) {
+            park[0] = m;
+            park[64] = l;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) park[64 * (2 + 16 * i + r)] = o[i][r];
+        }
+        __syncthreads();
+        if (grp == 1) return;
+        const float m2 = park[0], mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+        const float a1 = exp2_fast((m - ref) * sc2), a2 = exp2_fast((m2 - ref) * sc2);
+        m = mn;
+        l = l * a1 + park[64] * a2;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] = o[i][r] * a1 + park[64 * (2 + 16 * i + r)] * a2;
     }
     if (qi >= a.Tq) return;
     l = sum_halves(l);
@@ -750,7 +785,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
 }
 
 // ---------------------------------------------------------------------------------------------
-// Backward, queries: one workgroup = 128 queries; streams K / V.
+// Backward, queries: four waves x 32 queries (KG = 2: two waves for each 32 of 64, as in the forward
+// kernel); streams K / V.
 //
 // D = rowsum(dO * O) takes O as it was stored: rounded, and summed from rounded probabilities.
 // Its error is the same for all keys of a row, so it would come back as error * (P K) in dQ and
@@ -762,20 +798,20 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
 // Both backward kernels on 32 x 1024 x 12 heads of 64 with dropout: 335 us (160 + 175), bound like
 // the forward one; at 128 columns the accumulators leave one wave per SIMD (8 x 1024 x 16 heads:
 // 244 us), and a workgroup's time is 9 us + 1.2 us per 32 keys, which is what bounds ragged batches.
-template <class E, int DP, bool kDrop>
+template <class E, int DP, bool kDrop, int KG>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dq_kernel(AttnArgs a) {
-    constexpr int R = kStage, NB = DP / 32;
+    constexpr int R = kStage, NB = DP / 32, W = 4 / KG, kQueries = 32 * W;
     typedef Tile<E, DP, R> T;
     typedef typename T::x8 x8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int bh = shifted_head(a, a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
-    const int tile0 = (gridDim.y - 1 - blockIdx.y) * 128;
+    const int tile0 = (gridDim.y - 1 - blockIdx.y) * kQueries;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hh = lane >> 5;
     const Seq sq = sequence(a, b);
-    const int q0 = tile0 + wave * 32, qi = q0 + n;
+    const int grp = __builtin_amdgcn_readfirstlane(wave / W), q0 = tile0 + wave % W * 32, qi = q0 + n;
     const bool in = qi < sq.m;
-    const int stages = tile0 < sq.m ? (keys_seen(sq, min(tile0 + 127, sq.m - 1)) + R - 1) / R : 0;
+    const int stages = tile0 < sq.m ? (keys_seen(sq, min(tile0 + kQueries - 1, sq.m - 1)) + R - 1) / R : 0;
     const typename T::From kfrom = T::from(a.k, b * a.sk.b + hk * a.sk.h, a.sk.t, sq.n, a.D, tid);
     const typename T::From vfrom = T::from(a.v, b * a.sv.b + hk * a.sv.h, a.sv.t, sq.n, a.D, tid);
     const typename T::Lane at = T::lane_offsets(lane);
@@ -806,7 +842,8 @@ attn_dq_kernel(AttnArgs a) {
     const int seen_hi = __builtin_amdgcn_readfirstlane(q0 < sq.m ? keys_seen(sq, q0 + 31) : 0);
     const unsigned step = kDrop ? step_of(a) : 0u, head = static_cast<unsigned>(a.first_head + bh);
 
-    typename T::Regs kr, vr;
+    typename T::Regs kr[KG], vr[KG];
+    constexpr int kBuf = 2 * KG * T::kBytes;
     auto tile = [&](const char* Ks, const char* Vs, int key0) {
         f32x16 s = {0}, dp = {0};
 #pragma unroll
@@ -862,31 +899,63 @@ attn_dq_kernel(AttnArgs a) {
             }
         }
     };
-    auto stage = [&](int st, char* here, char* there) {
-        if (st + 1 < stages) {
-            kr = T::load(kfrom, st + 1);
-            vr = T::load(vfrom, st + 1);
+    auto fetch = [&](int it) {
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+            kr[g] = T::load(kfrom, it * KG + g);
+            vr[g] = T::load(vfrom, it * KG + g);
         }
+    };
+    auto put = [&](char* to) {
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+            T::store(to + 2 * g * T::kBytes, kr[g], tid);
+            T::store(to + (2 * g + 1) * T::kBytes, vr[g], tid);
+        }
+    };
+    const int turns = (stages + KG - 1) / KG;
+    auto turn = [&](int it, char* here, char* there) {
+        if (it + 1 < turns) fetch(it + 1);
+        const int st = it * KG + grp;
+        const char* at0 = here + 2 * grp * T::kBytes;
 #pragma unroll
         for (int sub = 0; sub < R / 32; ++sub)
             if (st * R + sub * 32 < seen_hi)  // wave-uniform
-                tile(here + sub * 32 * T::kRow, here + T::kBytes + sub * 32 * T::kRow, st * R + sub * 32);
-        if (st + 1 < stages) {
-            T::store(there, kr, tid);
-            T::store(there + T::kBytes, vr, tid);
-        }
+                tile(at0 + sub * 32 * T::kRow, at0 + T::kBytes + sub * 32 * T::kRow, st * R + sub * 32);
+        if (it + 1 < turns) put(there);
         __syncthreads();
     };
-    if (stages > 0) {
-        kr = T::load(kfrom, 0);
-        vr = T::load(vfrom, 0);
-        T::store(smem, kr, tid);
-        T::store(smem + T::kBytes, vr, tid);
+    if (turns > 0) {
+        fetch(0);
+        put(smem);
     }
     __syncthreads();
-    for (int st = 0; st < stages; st += 2) {
-        stage(st, smem, smem + 2 * T::kBytes);
-        if (st + 1 < stages) stage(st + 1, smem + 2 * T::kBytes, smem);
+    for (int it = 0; it < turns; it += 2) {
+        turn(it, smem, smem + kBuf);
+        if (it + 1 < turns) turn(it + 1, smem + kBuf, smem);
+    }
+    if (KG == 2) {
+        float* park = reinterpret_cast<float*>(smem) + (wave % W) * 64 * (NB * 32 + 1) + lane;
+        if (grp == 1) {
+            park[0] = off;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    park[64 * (1 + 32 * i + r)] = dq[i][r];
+                    park[64 * (17 + 32 * i + r)] = pk[i][r];
+                }
+        }
+        __syncthreads();
+        if (grp == 1) return;
+        off += park[0];
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dq[i][r] += park[64 * (1 + 32 * i + r)];
+                pk[i][r] += park[64 * (17 + 32 * i + r)];
+            }
     }
     if (qi >= a.Tq) return;
     off = sum_halves(off);
@@ -1131,11 +1200,35 @@ int set_lds(const void* fn, int bytes) {
     return hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? 0 : -20;
 }
 
-template <class E, int DP, bool kDrop>
+// Whether two waves share 32 queries (forward and dQ kernels): where the longest workgroup of a launch
+// takes longer than its CUs' share of the whole.  At 64 columns, two halves to a CU, up to 512
+// workgroups of 128 queries (1 x 4096, 12 heads: forward 75.6 -> 49.5 us, backward 167 -> 149; but 2 x
+// 4096: 84.7 -> 86.8), or 1024 if there are lengths, which leave some of them empty (six of 0 .. 777, 16
+// heads: 26.2 -> 20.9, 66 -> 60).  At 128, one half to a CU, below 256 (1 x 3624, 8 heads of 80: 88 -> 70,
+// 231 -> 196; but 4 x 512, 16 heads, which makes 256: 19.8 -> 22.9, 54 -> 58).
+bool halve_keys(const AttnArgs& a) {
+    const long groups = static_cast<long>(a.B) * a.H * ((a.Tq + 127) / 128);
+    const bool ragged = a.qlen != nullptr || a.klen != nullptr;
+    return a.Tk > 4 * kStage && (a.D > 64 ? groups < 256 : groups <= (ragged ? 1024 : 512));
+}
+
+template <class E, int DP, bool kDrop, int KG>
 int launch_fwd(const AttnArgs& a, hipStream_t s) {
-    constexpr int lds = 4 * Tile<E, DP, kStage>::kBytes;
-    if (const int st = set_lds(reinterpret_cast<const void*>(attn_fwd_kernel<E, DP, kDrop>), lds)) return st;
-    hipLaunchKernelGGL((attn_fwd_kernel<E, DP, kDrop>), dim3(a.B * a.H, (a.Tq + 127) / 128), dim3(256), lds, s, a);
+    constexpr int lds = 4 * KG * Tile<E, DP, kStage>::kBytes;  // (the joint needs less)
+    static_assert(KG == 1 || 2 * 64 * (DP / 2 + 2) * 4 <= lds, "room for the second waves' results");
+    if (const int st = set_lds(reinterpret_cast<const void*>(attn_fwd_kernel<E, DP, kDrop, KG>), lds)) return st;
+    hipLaunchKernelGGL((attn_fwd_kernel<E, DP, kDrop, KG>), dim3(a.B * a.H, (a.Tq + 128 / KG - 1) / (128 / KG)),
+                       dim3(256), lds, s, a);
+    return static_cast<int>(hipGetLastError());
+}
+
+template <class E, int DP, bool kDrop, int KG>
+int launch_dq(const AttnArgs& a, hipStream_t s) {
+    constexpr int ring = 4 * KG * Tile<E, DP, kStage>::kBytes, park = KG == 2 ? 2 * 64 * (DP + 1) * 4 : 0;
+    constexpr int lds = ring > park ? ring : park;
+    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop, KG>), lds)) return st;
+    hipLaunchKernelGGL((attn_dq_kernel<E, DP, kDrop, KG>), dim3(a.B * a.H, (a.Tq + 128 / KG - 1) / (128 / KG)),
+                       dim3(256), lds, s, a);
     return static_cast<int>(hipGetLastError());
 }
 
@@ -1174,13 +1267,11 @@ long delta_floats(const AttnArgs& a) { return (static_cast<long>(a.B) * a.H * a.
 
 template <class E, int DP, bool kDrop>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {
-    constexpr int rows = kStage;
-    constexpr int lds = 4 * Tile<E, DP, rows>::kBytes, lds2 = lds + 4 * rows * 4;
-    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop>), lds)) return st;
-    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dkdv_kernel<E, DP, kDrop>), lds2)) return st;
-    hipLaunchKernelGGL((attn_dq_kernel<E, DP, kDrop>), dim3(a.B * a.H, (a.Tq + 127) / 128), dim3(256), lds, s, a);
+    constexpr int lds = 4 * Tile<E, DP, kStage>::kBytes + 4 * kStage * 4;
+    if (const int st = halve_keys(a) ? launch_dq<E, DP, kDrop, 2>(a, s) : launch_dq<E, DP, kDrop, 1>(a, s)) return st;
+    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dkdv_kernel<E, DP, kDrop>), lds)) return st;
     hipLaunchKernelGGL((attn_dkdv_kernel<E, DP, kDrop>), dim3(a.B * a.Hk, (a.Tk + 127) / 128, a.splits), dim3(256),
-                       lds2, s, a);
+                       lds, s, a);
     if (a.splits > 1)
         hipLaunchKernelGGL((attn_add_kernel<E, DP>),
                            dim3(static_cast<unsigned>((2L * a.B * a.Hk * a.Tk * DP / 4 + 255) / 256)), dim3(256), 0, s, a);
@@ -1191,7 +1282,8 @@ template <class E, int DP>
 int launch(const AttnArgs& a, int backward, hipStream_t s) {
     if (backward) return a.limit ? launch_bwd<E, DP, true>(a, s) : launch_bwd<E, DP, false>(a, s);
     if (a.target >= 0) return launch_few<E, DP>(a, s);
-    return a.limit ? launch_fwd<E, DP, true>(a, s) : launch_fwd<E, DP, false>(a, s);
+    if (halve_keys(a)) return a.limit ? launch_fwd<E, DP, true, 2>(a, s) : launch_fwd<E, DP, false, 2>(a, s);
+    return a.limit ? launch_fwd<E, DP, true, 1>(a, s) : launch_fwd<E, DP, false, 1>(a, s);
 }
 
 bool fits(const void* p, const Strides& st) {

@@ -102,6 +102,17 @@ def test_few_queries_against_a_cache(Tq, Tk, H, Hk, D):
     check(*inputs(4, Tq, Tk, H, Hk, D, BF), BF, q_lengths=[min(Tq, n) for n in keys], k_lengths=keys, backward=False)
 
 
+@pytest.mark.parametrize("B,T,H,D", [(16, 260, 20, 64), (9, 300, 12, 128), (1, 1100, 2, 64), (1, 1061, 2, 128), (2, 513, 1, 40)])
+@pytest.mark.parametrize("causal,p", [(True, 0.1), (False, 0.0)])
+def test_many_and_few_tiles_of_queries(B, T, H, D, causal, p):
+    check(*inputs(B, T, T, H, H, D, FP), FP, causal=causal, p=p, seed=2)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_long_sequences_of_different_lengths(D):
+    check(*inputs(3, 600, 900, 2, 1, D, BF), BF, q_lengths=[600, 0, 333], k_lengths=[700, 900, 130], p=0.2, seed=4)
+
+
 def test_scores_far_apart_and_equal():
     q, k, v, dout = inputs(1, 96, 96, 2, 2, 64, BF)
     check(q * 8, k * 4, v, dout, BF, p=0.1)          # near one-hot rows

@@ -72,15 +72,18 @@ constexpr float kSlack = 8.f;
 struct Strides { long b, t, h; };  // elements between sequences, rows, heads
 
 struct AttnArgs {
-    const void *q, *k, *v;
-    void* out;
+    const void* q; Strides sq;
+    const void* k; Strides sk;
+    const void* v; Strides sv;
+    void* out; Strides so;
+    const void* dout; Strides sdo;
+    void* dq; Strides sdq;
+    void* dk; Strides sdk;
+    void* dv; Strides sdv;
     float* lse;               // [B][H][Tq]
-    const void* dout;
-    void *dq, *dk, *dv;
     float* delta;             // [B][H][Tq], rowsum(dO * O): written by the dQ kernel
     const int *qlen, *klen;   // [B] or null
     const long* step_at;
-    Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
     unsigned long seed;
     unsigned long first_head; // number of the first head of the mask's counter
     int B, Tq, Tk, H, Hk, D, causal;

@@ -627,7 +627,8 @@ class GPT2NativeTrainer(GroupTrainer):
         the embedding gradient) are assembled on the host for the whole round - the host
         holds a copy of the token shard and draws the shuffles itself - and copied into the
         graph's static input buffers before each replay; the captured step holds no sort,
-        no gather and no allocation.  The first step of a (first client, group size) pair
+        no gather and no allocation (with embedding dropout it holds the sort and the scratch
+        memory of that operator's gradient).  The first step of a (first client, group size) pair
         runs eagerly on the same buffers (it warms the workspaces up), the second is
         captured, every later one is a replay."""
         cfg = self.cfg

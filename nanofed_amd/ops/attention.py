@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import struct
 from ctypes import c_int, c_long, c_void_p
+from functools import lru_cache
 
 import torch
 import torch.nn.functional as F
@@ -133,10 +134,10 @@ def causal_attention_bwd(qkv: torch.Tensor, out: torch.Tensor, lse: torch.Tensor
 MAX_HEAD_DIM = 128
 _TYPES = {torch.bfloat16: 1, torch.float16: 2}
 
-# ``AttnArgs`` of csrc/hip/attention_general.hip: addresses (q k v out lse dout dq dk dv delta, the
-# lengths, the step in memory), distances between sequences, rows and heads (q k v out dout dq dk
-# dv), seed and first head, sizes, scale and factor of what is kept, threshold and step, scratch
-_PACK = struct.Struct("@13P24q2Q7i2f2IP2i0q")
+# ``AttnArgs`` of csrc/hip/attention_general.hip: q k v out dout dq dk dv, each an address and the
+# distances between sequences, rows and heads; addresses of lse, delta, the lengths and the step in
+# memory; seed and first head, sizes, scale and factor of what is kept, threshold and step, scratch
+_PACK = struct.Struct("@" + "P3q" * 8 + "5P2Q7i2f2IP2i0q")
 _NONE = (0, 0, 0, 0)
 
 
@@ -148,19 +149,24 @@ class _Args:
 
     def pack(self, lse: int, out: tuple, dout=_NONE, dq=_NONE, dk=_NONE, dv=_NONE, delta: int = 0,
              parts: int = 0) -> bytes:
-        q, k, v = self.q, self.k, self.v
         return _PACK.pack(
-            q[0], k[0], v[0], out[0], lse, dout[0], dq[0], dk[0], dv[0], delta, self.qlen, self.klen,
-            self.step_at, *q[1:], *k[1:], *v[1:], *out[1:], *dout[1:], *dq[1:], *dk[1:], *dv[1:],
-            self.seed, self.first_head, self.B, self.Tq, self.Tk, self.H, self.Hk, self.D, self.causal,
-            self.scale, self.up, self.limit, self.step, parts, 0, 0)
+            *self.q, *self.k, *self.v, *out, *dout, *dq, *dk, *dv, lse, delta, self.qlen, self.klen,
+            self.step_at, self.seed, self.first_head, self.B, self.Tq, self.Tk, self.H, self.Hk, self.D,
+            self.causal, self.scale, self.up, self.limit, self.step, parts, 0, 0)
 
 
-def _operand(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, written: bool) -> tuple:
+@lru_cache(maxsize=1024)
+def _scratch_floats(backward: bool, B: int, Tq: int, Tk: int, H: int, Hk: int, D: int, limit: int) -> int:
+    sizes = _PACK.pack(*_NONE * 8, 0, 0, 0, 0, 0, 0, 0, B, Tq, Tk, H, Hk, D, 0, 1.0, 1.0, limit, 0, 0, 0, 0)
+    return _fn("nf_attention_bwd_floats" if backward else "nf_attention_fwd_floats")(sizes)
+
+
+def _operand(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, dev: torch.device,
+             written: bool) -> tuple:
     """Checks a ``[B, T, heads, D]`` operand; its address and the distances between its sequences,
     rows and heads."""
-    if t.dtype is not like.dtype or t.device != like.device:
-        raise DeviceError(f"attention: {name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if t.dtype is not dtype or t.device != dev:
+        raise DeviceError(f"attention: {name} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise DeviceError(f"attention: {name} must be {list(shape)}, got {list(t.shape)}")
     at = t.data_ptr()
@@ -207,9 +213,10 @@ def _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step
     a.scale = scale = D**-0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise DeviceError("attention: the scale must be positive")
-    a.limit = limit_of(dropout, 8, "attention")
+    a.limit = limit_of(dropout, 8, "attention") if dropout else 0
     a.up = 256 / (256 - a.limit)
-    check_key(seed, step, q.device, "attention")
+    dtype, dev = q.dtype, q.device
+    check_key(seed, step, dev, "attention")
     a.seed = seed
     a.step_at, a.step = (step.data_ptr(), 0) if isinstance(step, torch.Tensor) else (0, step)
     if not 0 <= first_batch < 1 << 32:
@@ -217,17 +224,17 @@ def _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step
     a.first_head = first_batch * H
     a.causal = bool(causal)
     shared = (B, Tk, Hk, D)
-    a.q = _operand(q, "q", shape, q, False)
-    a.k = _operand(k, "k", shared, q, False)
-    a.v = _operand(v, "v", shared, q, False)
+    a.q = _operand(q, "q", shape, dtype, dev, False)
+    a.k = _operand(k, "k", shared, dtype, dev, False)
+    a.v = _operand(v, "v", shared, dtype, dev, False)
     a.qlen, a.klen = _lengths(q_lengths, "q_lengths", q), _lengths(k_lengths, "k_lengths", q)
     return a
 
 
-def _check_lse(lse: torch.Tensor, a: _Args, q: torch.Tensor) -> None:
-    if (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device
+def _check_lse(lse: torch.Tensor, a: _Args, dev: torch.device) -> None:
+    if (lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.device != dev
             or lse.shape != (a.B, a.H, a.Tq)):
-        raise DeviceError(f"attention: lse must be contiguous float32 [{a.B}, {a.H}, {a.Tq}] on {q.device}")
+        raise DeviceError(f"attention: lse must be contiguous float32 [{a.B}, {a.H}, {a.Tq}] on {dev}")
 
 
 def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor | None = None,
@@ -261,8 +268,9 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if lse is None:
         lse = q.new_empty((a.B, a.H, a.Tq), dtype=torch.float32)
-    to = _operand(out, "out", q.shape, q, True)
-    _check_lse(lse, a, q)
+    dev = q.device
+    to = _operand(out, "out", q.shape, q.dtype, dev, True)
+    _check_lse(lse, a, dev)
     if a.B == 0 or a.Tq == 0:
         return out, lse
     if a.Tk == 0:
@@ -275,14 +283,12 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
         y = (prob * kept) @ _shared(a, v, k_lengths)
         out.copy_(y.transpose(1, 2))
         return out, lse
-    packed, dev = a.pack(lse.data_ptr(), to), q.device
+    # (scratch of its own for every call: the allocator hands it on in stream order, and a captured
+    # call's belongs to its graph)
+    floats = _scratch_floats(False, a.B, a.Tq, a.Tk, a.H, a.Hk, a.D, a.limit)
+    parts = q.new_empty(floats, dtype=torch.float32) if floats else None
+    packed = a.pack(lse.data_ptr(), to, parts=parts.data_ptr() if floats else 0)
     with library.on_device(dev):
-        floats = _fn("nf_attention_fwd_floats")(packed)
-        if floats:
-            # (scratch of its own for every call: the allocator hands it on in stream order, and a
-            # captured call's belongs to its graph)
-            parts = q.new_empty(floats, dtype=torch.float32)
-            packed = a.pack(lse.data_ptr(), to, parts=parts.data_ptr())
         library.check(_fn("nf_attention")(packed, _TYPES[q.dtype], 0, library.stream_ptr(dev)), "attention_fwd")
     return out, lse
 
@@ -299,11 +305,11 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     that share it in a fixed order, without atomics.  ``dq``, ``dk``, ``dv`` must not overlap what is
     read."""
     a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
-    shape, shared = q.shape, k.shape
-    operands = (_operand(out, "out", shape, q, False), _operand(dout, "dout", shape, q, False),
-                _operand(dq, "dq", shape, q, True), _operand(dk, "dk", shared, q, True),
-                _operand(dv, "dv", shared, q, True))
-    _check_lse(lse, a, q)
+    shape, shared, dtype, dev = q.shape, k.shape, q.dtype, q.device
+    operands = (_operand(out, "out", shape, dtype, dev, False), _operand(dout, "dout", shape, dtype, dev, False),
+                _operand(dq, "dq", shape, dtype, dev, True), _operand(dk, "dk", shared, dtype, dev, True),
+                _operand(dv, "dv", shared, dtype, dev, True))
+    _check_lse(lse, a, dev)
     if a.B == 0 or a.Tq == 0 or a.Tk == 0:
         for t in (dq, dk, dv):
             t.zero_()
@@ -320,12 +326,10 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
         for t, g in ((dk, ds.transpose(-1, -2) @ qf), (dv, gv)):
             t.copy_(g.view(a.B, a.Hk, a.H // a.Hk, a.Tk, a.D).sum(2).transpose(1, 2))
         return
-    dev = q.device
+    scratch = q.new_empty(_scratch_floats(True, a.B, a.Tq, a.Tk, a.H, a.Hk, a.D, a.limit), dtype=torch.float32)
+    packed = a.pack(lse.data_ptr(), *operands, delta=scratch.data_ptr())
     with library.on_device(dev):
-        floats = _fn("nf_attention_bwd_floats")(a.pack(0, _NONE))
-        scratch = q.new_empty(floats, dtype=torch.float32)
-        library.check(_fn("nf_attention")(a.pack(lse.data_ptr(), *operands, delta=scratch.data_ptr()),
-                                          _TYPES[q.dtype], 1, library.stream_ptr(dev)), "attention_bwd")
+        library.check(_fn("nf_attention")(packed, _TYPES[dtype], 1, library.stream_ptr(dev)), "attention_bwd")
 
 
 def _valid(a: _Args, lengths: torch.Tensor | None, T: int) -> torch.Tensor:

@@ -496,9 +496,9 @@ attn_fwd_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Forward of few queries (queries x heads per key head <= 32) against many keys: the queries of
-// all heads that share a key head are the columns of one tile, so the keys are read once for all
-// of them.  Bound by reading the keys and values.  A workgroup takes a chunk of the keys, its
+// Forward of few queries against many keys: the queries of all heads that share a key head are the
+// columns of one tile of 32, so the keys are read once for all of them (more than 32: once for each
+// tile, blockIdx.y).  Bound by reading the keys and values.  A workgroup takes a chunk of the keys, its
 // waves every fourth 32 of them, through LDS of their own (no barrier in the loop), one tile ahead
 // in registers.  The waves are joined through LDS, the chunks by attn_join_kernel.
 //
@@ -509,7 +509,7 @@ attn_fwd_kernel(AttnArgs a) {
 // 19.0 us + 5.4 us for the join with 512 workgroups, 4.4 TB/s; 23.0 + 4.9 with 256; without the
 // hint that the keys are read once, which leaves the parts in L2, 20.2 + 6.2.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-constexpr int kFew = 32, kFewMaxBatch = 512, kFewTarget = 512;
+constexpr int kFewQueries = 32, kFewRows = 256, kFewMaxBatch = 512, kFewTarget = 512;
 constexpr int kOnce = 2;  // non-temporal load
 
 struct Chunk { int b, hk, count, at, size; Seq seq; };  // chunk `at` of `count` of (b, hk), keys per chunk
@@ -571,7 +571,8 @@ attn_few_kernel(AttnArgs a) {
     if (me.b < 0) return;
     const int b = me.b, hk = me.hk, group = a.H / a.Hk;
     const Seq sq = me.seq;
-    const int rows = a.Tq * group, qi = n / group, h = hk * group + n % group;
+    const int row0 = 32 * blockIdx.y, all = a.Tq * group, rows = min(32, all - row0);  // of this tile
+    const int qi = (row0 + n) / group, h = hk * group + (row0 + n) % group;
     const bool in = n < rows && qi < sq.m;
     const int seen = (in ? keys_seen(sq, qi) : 0) - 4 * hh;
     const int k0 = me.at * me.size, k1 = min(sq.m > 0 ? sq.n : 0, k0 + me.size);
@@ -679,7 +680,7 @@ attn_few_kernel(AttnArgs a) {
             }
     }
     __syncthreads();
-    const long parts = static_cast<long>(gridDim.x) * rows;
+    const long parts = static_cast<long>(gridDim.x) * all;
     for (int idx = threadIdx.x; idx < rows * kPieces; idx += 256) {
         const int row = idx / kPieces, piece = idx % kPieces, col = 4 * piece;
         float mw[4], top = -INFINITY, sum = 0.f;
@@ -697,12 +698,12 @@ attn_few_kernel(AttnArgs a) {
             for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], f, v[e]);
         }
         if (me.count > 1) {
-            const long part = static_cast<long>(blockIdx.x) * rows + row;
+            const long part = static_cast<long>(blockIdx.x) * all + row0 + row;
             *reinterpret_cast<f32x4*>(a.parts + part * DP + col) = v;
             if (piece == 0) *reinterpret_cast<f32x2*>(a.parts + parts * DP + 2 * part) = f32x2{top, sum};
             continue;
         }
-        const int qr = row / group, head = hk * group + row % group;
+        const int qr = (row0 + row) / group, head = hk * group + (row0 + row) % group;
         const bool some = qr < sq.m && (sum > 0.f || sum != sum);
         const float inv = some ? 1.f / sum : 0.f;
         if (col < a.D) {
@@ -1237,9 +1238,18 @@ int launch_dq(const AttnArgs& a, hipStream_t s) {
 
 // Workgroups that attn_few_kernel cuts the keys for (0: one per sequence and key head; -1: not the
 // few-query form).
+// More than one tile reads the keys once for each, the form for many queries once for each head, with
+// one of four waves at work: several tiles pay against long caches where they are at most half as many
+// as the heads that share a key head, or where there are few heads for the chip.  (8191 keys, 5 queries,
+// 64 heads on 8 of 128, B 4: 48 us, 220 by head; 1024 keys, 32 queries, 32 heads on 4, B 2: 18, 24; but
+// 48 heads on 12 of 64, B 8: 30, 21; 512 keys, 5 queries, 64 heads on 8 of 64, B 4: 14.7, 10.9.)
+int few_tiles(const AttnArgs& a) { return (a.Tq * (a.H / a.Hk) + 31) / 32; }
 int few_target(const AttnArgs& a) {
-    if (a.limit != 0 || static_cast<long>(a.Tq) * (a.H / a.Hk) > kFew) return -1;
-    return a.B <= kFewMaxBatch && a.B * a.Hk < kFewTarget && a.Tk > 128 ? kFewTarget : 0;
+    const int group = a.H / a.Hk;
+    if (a.limit != 0 || a.Tq > kFewQueries || group > kFewRows || a.Tq * group > kFewRows) return -1;
+    const int tiles = few_tiles(a), target = kFewTarget / tiles;
+    if (tiles > 1 && (a.Tk < 1024 || (2 * tiles > group && static_cast<long>(a.B) * a.H > 128))) return -1;
+    return a.B <= kFewMaxBatch && static_cast<long>(a.B) * a.Hk < target && a.Tk > 128 ? target : 0;
 }
 int few_workgroups(const AttnArgs& a) { return a.target + a.B * a.Hk; }  // at most
 int padded_dim(int D) { return D <= 64 ? 64 : 128; }
@@ -1249,7 +1259,7 @@ int launch_few(const AttnArgs& a, hipStream_t s) {
     constexpr int lds = 8 * Tile<E, DP, 32>::kBytes + 4 * 64 * 4;
     if (a.target != 0 && a.parts == nullptr) return -2;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_few_kernel<E, DP>), lds)) return st;
-    hipLaunchKernelGGL((attn_few_kernel<E, DP>), dim3(few_workgroups(a)), dim3(256), lds, s, a);
+    hipLaunchKernelGGL((attn_few_kernel<E, DP>), dim3(few_workgroups(a), few_tiles(a)), dim3(256), lds, s, a);
     if (a.target != 0)
         hipLaunchKernelGGL((attn_join_kernel<E, DP>), dim3((a.B * a.H * a.Tq + 3) / 4), dim3(256), 0, s, a,
                            few_workgroups(a));

@@ -102,6 +102,13 @@ def test_few_queries_against_a_cache(Tq, Tk, H, Hk, D):
     check(*inputs(4, Tq, Tk, H, Hk, D, BF), BF, q_lengths=[min(Tq, n) for n in keys], k_lengths=keys, backward=False)
 
 
+@pytest.mark.parametrize("Tq,Tk,H,Hk", [(5, 700, 8, 1), (5, 1030, 14, 2), (32, 1024, 8, 1), (33, 1100, 1, 1), (9, 1500, 28, 1), (1, 1200, 160, 2)])
+@pytest.mark.parametrize("causal,dtype,D", [(True, BF, 64), (False, FP, 128)])
+def test_few_queries_of_many_heads_against_a_cache(Tq, Tk, H, Hk, causal, dtype, D):
+    check(*inputs(3, Tq, Tk, H, Hk, D, dtype), dtype, q_lengths=[Tq, Tq // 2, Tq], k_lengths=[Tk, Tk // 3, 1],
+          causal=causal, backward=False)
+
+
 @pytest.mark.parametrize("B,T,H,D", [(16, 260, 20, 64), (9, 300, 12, 128), (1, 1100, 2, 64), (1, 1061, 2, 128), (2, 513, 1, 40)])
 @pytest.mark.parametrize("causal,p", [(True, 0.1), (False, 0.0)])
 def test_many_and_few_tiles_of_queries(B, T, H, D, causal, p):

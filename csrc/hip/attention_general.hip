@@ -194,6 +194,15 @@ __device__ __forceinline__ typename Vec<E>::x8 pack8(const f32x16& v, int first)
     return o;
 }
 
+// what pack8 rounds away
+template <class E>
+__device__ __forceinline__ typename Vec<E>::x8 rest8(const f32x16& v, int first) {
+    typename Vec<E>::x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = static_cast<E>(v[first + j] - static_cast<float>(static_cast<E>(v[first + j])));
+    return o;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // -- the dropout mask of a 32 x 32 tile -------------------------------------------------------
@@ -802,7 +811,11 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
 // Both backward kernels on 32 x 1024 x 12 heads of 64 with dropout: 335 us (160 + 175), bound like
 // the forward one; at 128 columns the accumulators leave one wave per SIMD (8 x 1024 x 16 heads:
 // 244 us), and a workgroup's time is 9 us + 1.2 us per 32 keys, which is what bounds ragged batches.
-template <class E, int DP, bool kDrop, int KG>
+//
+// kFine: P and dS are rounded to the operands' type for the products, an error like that of rounding
+// the results, so that the two add up to sqrt(2) of one over many terms.  Over few a sum can come out
+// worse; then the rounding is undone by a product with what it left (see fine).
+template <class E, int DP, bool kDrop, int KG, bool kFine>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dq_kernel(AttnArgs a) {
     constexpr int R = kStage, NB = DP / 32, W = 4 / KG, kQueries = 32 * W;
@@ -902,6 +915,14 @@ attn_dq_kernel(AttnArgs a) {
                 pk[i] = mma(kt[g][i], p, pk[i]);
             }
         }
+        if (kFine) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const x8 ds = rest8<E>(dp, 8 * g);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) dq[i] = mma(kt[g][i], ds, dq[i]);
+            }
+        }
     };
     auto fetch = [&](int it) {
 #pragma unroll
@@ -986,7 +1007,7 @@ attn_dq_kernel(AttnArgs a) {
 // all heads are cut into ranges (key_plan), one workgroup each (blockIdx.z): they leave fp32 sums in
 // `parts` ([range][dK, dV][B][Hk][Tk][DP]) that attn_add_kernel adds in order.  (6 ragged sequences
 // of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 57 + 9 us in ranges.)
-template <class E, int DP, bool kDrop>
+template <class E, int DP, bool kDrop, bool kFine>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dkdv_kernel(AttnArgs a) {
     constexpr int R = kStage, NB = DP / 32;
@@ -1105,6 +1126,17 @@ attn_dkdv_kernel(AttnArgs a) {
                 for (int i = 0; i < NB; ++i) {
                     dv[i] = mma(p, dt[k][i], dv[i]);
                     dk[i] = mma(ds, qt[k][i], dk[i]);
+                }
+            }
+            if (kFine) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const x8 p = rest8<E>(pd, 8 * k), ds = rest8<E>(dp, 8 * k);
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        dv[i] = mma(p, dt[k][i], dv[i]);
+                        dk[i] = mma(ds, qt[k][i], dk[i]);
+                    }
                 }
             }
         };
@@ -1226,12 +1258,12 @@ int launch_fwd(const AttnArgs& a, hipStream_t s) {
     return static_cast<int>(hipGetLastError());
 }
 
-template <class E, int DP, bool kDrop, int KG>
+template <class E, int DP, bool kDrop, int KG, bool kFine>
 int launch_dq(const AttnArgs& a, hipStream_t s) {
     constexpr int ring = 4 * KG * Tile<E, DP, kStage>::kBytes, park = KG == 2 ? 2 * 64 * (DP + 1) * 4 : 0;
     constexpr int lds = ring > park ? ring : park;
-    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop, KG>), lds)) return st;
-    hipLaunchKernelGGL((attn_dq_kernel<E, DP, kDrop, KG>), dim3(a.B * a.H, (a.Tq + 128 / KG - 1) / (128 / KG)),
+    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop, KG, kFine>), lds)) return st;
+    hipLaunchKernelGGL((attn_dq_kernel<E, DP, kDrop, KG, kFine>), dim3(a.B * a.H, (a.Tq + 128 / KG - 1) / (128 / KG)),
                        dim3(256), lds, s, a);
     return static_cast<int>(hipGetLastError());
 }
@@ -1278,12 +1310,19 @@ int key_splits(const AttnArgs& a) {
 }
 long delta_floats(const AttnArgs& a) { return (static_cast<long>(a.B) * a.H * a.Tq + 3) & ~3L; }
 
-template <class E, int DP, bool kDrop>
+// Whether the backward pass undoes the rounding of P and dS: sequences of up to 128 (where it costs least,
+// 32 x 128 x 12 heads of 64: 28.1 -> 30.5 us, one sequence of 33: nothing), and longer ones of few heads.
+// (Error of dQ over that of rounding alone: 1.0; without it 1.35 .. 1.7 at lengths of 4, 1.45 at 192.)
+bool fine(const AttnArgs& a) {
+    return (a.Tq <= 128 && a.Tk <= 128) || static_cast<double>(a.B) * a.H * a.Tq * a.Tk <= 262144.0;
+}
+
+template <class E, int DP, bool kDrop, bool kFine>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {
     constexpr int lds = 4 * Tile<E, DP, kStage>::kBytes + 4 * kStage * 4;
-    if (const int st = halve_keys(a) ? launch_dq<E, DP, kDrop, 2>(a, s) : launch_dq<E, DP, kDrop, 1>(a, s)) return st;
-    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dkdv_kernel<E, DP, kDrop>), lds)) return st;
-    hipLaunchKernelGGL((attn_dkdv_kernel<E, DP, kDrop>), dim3(a.B * a.Hk, (a.Tk + 127) / 128, a.splits), dim3(256),
+    if (const int st = !kFine && halve_keys(a) ? launch_dq<E, DP, kDrop, 2, false>(a, s) : launch_dq<E, DP, kDrop, 1, kFine>(a, s)) return st;
+    if (const int st = set_lds(reinterpret_cast<const void*>(attn_dkdv_kernel<E, DP, kDrop, kFine>), lds)) return st;
+    hipLaunchKernelGGL((attn_dkdv_kernel<E, DP, kDrop, kFine>), dim3(a.B * a.Hk, (a.Tk + 127) / 128, a.splits), dim3(256),
                        lds, s, a);
     if (a.splits > 1)
         hipLaunchKernelGGL((attn_add_kernel<E, DP>),
@@ -1293,7 +1332,8 @@ int launch_bwd(const AttnArgs& a, hipStream_t s) {
 
 template <class E, int DP>
 int launch(const AttnArgs& a, int backward, hipStream_t s) {
-    if (backward) return a.limit ? launch_bwd<E, DP, true>(a, s) : launch_bwd<E, DP, false>(a, s);
+    if (backward && fine(a)) return a.limit ? launch_bwd<E, DP, true, true>(a, s) : launch_bwd<E, DP, false, true>(a, s);
+    if (backward) return a.limit ? launch_bwd<E, DP, true, false>(a, s) : launch_bwd<E, DP, false, false>(a, s);
     if (a.target >= 0) return launch_few<E, DP>(a, s);
     if (halve_keys(a)) return a.limit ? launch_fwd<E, DP, true, 2>(a, s) : launch_fwd<E, DP, false, 2>(a, s);
     return a.limit ? launch_fwd<E, DP, true, 1>(a, s) : launch_fwd<E, DP, false, 1>(a, s);

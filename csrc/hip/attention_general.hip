@@ -568,7 +568,7 @@ __device__ __forceinline__ Chunk few_chunk(const AttnArgs& a, int id, int lane) 
 }
 
 template <class E, int DP, bool kFine>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 && kFine ? 1 : 2)))
 attn_few_kernel(AttnArgs a) {
     typedef Tile<E, DP, 32> T;
     typedef typename T::x8 x8;
@@ -663,12 +663,15 @@ attn_few_kernel(AttnArgs a) {
         const x8 p0 = pack8<E>(s, 0), p1 = pack8<E>(s, 8);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const x8 v0 = T::tr(lds + T::kBytes, at, 0, i), v1 = T::tr(lds + T::kBytes, at, 16, i);
-            o[i] = mma(v0, p0, o[i]);
-            o[i] = mma(v1, p1, o[i]);
-            if (kFine) {  // what the rounding of P leaves
-                o[i] = mma(v0, rest8<E>(s, 0), o[i]);
-                o[i] = mma(v1, rest8<E>(s, 8), o[i]);
+            o[i] = mma(T::tr(lds + T::kBytes, at, 0, i), p0, o[i]);
+            o[i] = mma(T::tr(lds + T::kBytes, at, 16, i), p1, o[i]);
+        }
+        if (kFine) {  // what the rounding of P leaves
+            const x8 r0 = rest8<E>(s, 0), r1 = rest8<E>(s, 8);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                o[i] = mma(T::tr(lds + T::kBytes, at, 0, i), r0, o[i]);
+                o[i] = mma(T::tr(lds + T::kBytes, at, 16, i), r1, o[i]);
             }
         }
     }
@@ -1013,7 +1016,7 @@ attn_dq_kernel(AttnArgs a) {
 // `parts` ([range][dK, dV][B][Hk][Tk][DP]) that attn_add_kernel adds in order.  (6 ragged sequences
 // of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 57 + 9 us in ranges.)
 template <class E, int DP, bool kDrop, bool kFine>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 && !kFine ? 2 : 1)))
 attn_dkdv_kernel(AttnArgs a) {
     constexpr int R = kStage, NB = DP / 32;
     typedef Tile<E, DP, R> T;
@@ -1320,12 +1323,11 @@ int key_splits(const AttnArgs& a) {
 }
 long delta_floats(const AttnArgs& a) { return (static_cast<long>(a.B) * a.H * a.Tq + 3) & ~3L; }
 
-// Whether the backward pass undoes the rounding of P and dS: sequences of up to 128 (where it costs least,
-// 32 x 128 x 12 heads of 64: 28.1 -> 30.5 us, one sequence of 33: nothing), and longer ones of few heads.
-// (Error of dQ over that of rounding alone: 1.0; without it 1.35 .. 1.7 at lengths of 4, 1.45 at 192.)
-bool fine(const AttnArgs& a) {
-    return (a.Tq <= 128 && a.Tk <= 128) || static_cast<double>(a.B) * a.H * a.Tq * a.Tk <= 262144.0;
-}
+// Whether the backward pass undoes the rounding of P and dS: where there are so few pairs that the errors
+// do not average.  (Error of dQ over that of rounding alone: 1.0; without it 1.35 .. 1.7 at a few short
+// sequences, 1.41 .. 1.44 at many.  One sequence of 33: the same time; it would cost 32 sequences of 128,
+// 12 heads of 64, 28 -> 37 us.)
+bool fine(const AttnArgs& a) { return static_cast<double>(a.B) * a.H * a.Tq * a.Tk <= 524288.0; }
 
 template <class E, int DP, bool kDrop, bool kFine>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {

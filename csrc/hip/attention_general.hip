@@ -69,6 +69,21 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // multiplied by at nearly every tile (some of 32 rows finds a new maximum) is spared.
 constexpr float kSlack = 8.f;
 
+// Half has the exponents 2^-14 .. 2^15 (2^-24 with fewer bits), and the factors P and dS = P (dP - D) of the
+// gradients leave them long before the gradients do: P is 1 / keys, dS that times dO.  So the backward
+// kernels hold P times 2^kProb, which a probability cannot carry beyond the type, and dS times a power of
+// two on top, which the dQ kernel finds for every query from what it meets (GradScale), the dK / dV kernel for
+// its workgroup from what the dQ kernel left (bounds).  Both are exact and are taken out in fp32.  bf16
+// has the exponents of fp32 and needs neither.
+template <class E> struct Exponent {
+    static constexpr bool kScaled = false;
+    static constexpr float kProb = 0.f, kUnprob = 1.f;  // 2^-kProb
+};
+template <> struct Exponent<half> {
+    static constexpr bool kScaled = true;
+    static constexpr float kProb = 15.f, kUnprob = 1.f / 32768.f;
+};
+
 struct Strides { long b, t, h; };  // elements between sequences, rows, heads
 
 struct AttnArgs {
@@ -81,7 +96,7 @@ struct AttnArgs {
     void* dk; Strides sdk;
     void* dv; Strides sdv;
     float* lse;               // [B][H][Tq]
-    float* delta;             // [B][H][Tq], rowsum(dO * O): written by the dQ kernel
+    float* delta;             // [B][H][Tq], rowsum(dO * O): written by the dQ kernel; bounds behind it
     const int *qlen, *klen;   // [B] or null
     const long* step_at;
     unsigned long seed;
@@ -226,6 +241,31 @@ __device__ __forceinline__ void quad_transpose(unsigned (&w)[4], int lane) {
     }
 }
 
+// The factor of a query's dS: so that the largest one of the first tile with any lies in [2^6, 2^7), and
+// room for those that are up to 2^8 times larger; where a tile holds one beyond that, what was summed so far
+// is multiplied too.  (A narrower room costs: with a factor of 4 some of a wave's 32 rows pass it at every
+// sixth tile or so, and the dQ kernel of six sequences of up to 777 takes 58 us instead of 55; without any of this it takes 49.5,
+// the dK / dV kernel 61 instead of 63.)
+struct GradScale {
+    float x = 1.f, limit = 0.f, top = 0.f;  // |dS * x| up to `top` so far, `limit` allowed (0: all dS so far are 0)
+
+    // The further factor for a tile whose largest |dS * x| of this query is `most`.
+    __device__ __forceinline__ float grow(float most) {
+        if (!(most > limit)) return 1.f;  // (also a NaN)
+        if (most == INFINITY) {           // the row's gradient is not finite, whatever the factor
+            limit = INFINITY;
+            return 1.f;
+        }
+        // (at most 2^60: with it no dO V^T of half operands passes the range of fp32)
+        const float f = ldexpf(1.f, min(7 - __builtin_amdgcn_frexp_expf(most), 60));
+        x *= f;
+        top *= f;
+        limit = 32768.f;
+        return f;
+    }
+    __device__ __forceinline__ bool set() const { return limit == 32768.f; }
+};
+
 // Bytes of the lane's 16 probabilities, four per word: byte e of word g belongs to accumulator
 // register 4 g + e.  kKeysInRows: the rows of the tile are keys (row0 = first key, col0 = first
 // query), else queries.
@@ -273,6 +313,17 @@ __device__ __forceinline__ float max_halves(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// of all lanes
+__device__ __forceinline__ float max_wave(float v) {
+    auto with = [&](unsigned other) { v = fmaxf(v, __uint_as_float(other)); };
+    with(quad<0xB1>(__float_as_uint(v)));   // lane ^ 1
+    with(quad<0x4E>(__float_as_uint(v)));   // lane ^ 2
+    with(quad<0x141>(__float_as_uint(v)));  // the other four of eight, mirrored
+    with(quad<0x140>(__float_as_uint(v)));  // the other eight of sixteen, mirrored
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return max_halves(v);
+}
 __device__ __forceinline__ float sum_halves(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
@@ -315,6 +366,15 @@ __device__ __forceinline__ KeyPlan key_plan(const AttnArgs& a, const Seq& s, int
 __device__ __forceinline__ int shifted_head(const AttnArgs& a, int heads) {
     if (a.klen == nullptr && a.qlen == nullptr) return blockIdx.x;
     return static_cast<int>((blockIdx.x + static_cast<unsigned long>(heads) * blockIdx.y) % gridDim.x);
+}
+
+__host__ __device__ __forceinline__ long delta_floats(const AttnArgs& a) {
+    return (static_cast<long>(a.B) * a.H * a.Tq + 3) & ~3L;
+}
+// Behind delta: for every 32 queries of a head a bound of 2^kProb |dS| (half).
+__host__ __device__ __forceinline__ int bounds_of_head(const AttnArgs& a) { return (a.Tq + 31) / 32; }
+__host__ __device__ __forceinline__ long bound_floats(const AttnArgs& a) {
+    return (static_cast<long>(a.B) * a.H * bounds_of_head(a) + 3) & ~3L;
 }
 
 __device__ __forceinline__ unsigned step_of(const AttnArgs& a) {
@@ -827,6 +887,7 @@ template <class E, int DP, bool kDrop, int KG, bool kFine>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dq_kernel(AttnArgs a) {
     constexpr int R = kStage, NB = DP / 32, W = 4 / KG, kQueries = 32 * W;
+    typedef Exponent<E> X;
     typedef Tile<E, DP, R> T;
     typedef typename T::x8 x8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -857,7 +918,9 @@ attn_dq_kernel(AttnArgs a) {
     const long row = static_cast<long>(bh) * a.Tq + qi;
     // a row that sees no key has lse -inf: +inf makes its probabilities 0
     float lse2 = in ? a.lse[row] : -INFINITY;
-    lse2 = lse2 == -INFINITY ? INFINITY : lse2 * kLog2e;
+    lse2 = lse2 == -INFINITY ? INFINITY : lse2 * kLog2e - X::kProb;
+    GradScale gs;
+    float up = kDrop ? a.up : 1.f, xdelta = delta;  // times gs.x
     f32x16 dq[NB], pk[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) { dq[i] = f32x16{0}; pk[i] = f32x16{0}; }
@@ -897,7 +960,8 @@ attn_dq_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s[r] = exp2_fast(fmaf(s[r], sc2, -lse2));
-            if (kDrop) dp[r] = fmaf(dp[r], kept(w, r, a.limit) ? a.up : 0.f, -delta);
+            if (kDrop) dp[r] = fmaf(dp[r], kept(w, r, a.limit) ? up : 0.f, -xdelta);
+            else if (X::kScaled) dp[r] = fmaf(dp[r], up, -xdelta);
             else dp[r] -= delta;
         }
         if (key0 + 32 > seen_lo) {  // wave-uniform: some pair of the tile is not visible
@@ -907,12 +971,33 @@ attn_dq_kernel(AttnArgs a) {
             for (int r = 0; r < 16; ++r)
                 if (reg_row(r) >= lim) { s[r] = 0.f; dp[r] = 0.f; }
         }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+        if (X::kScaled) {
+            float some[4] = {0.f, 0.f, 0.f, 0.f};  // (four short chains)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) some[r & 3] = fmaxf(some[r & 3], fabsf(dp[r]));
+            float most = fmaxf(fmaxf(some[0], some[1]), fmaxf(some[2], some[3]));
+            if (__any(most > gs.limit)) {
+                keep_branch();
+                most = max_halves(most);  // (both halves of a query take the same factor)
+                const float f = gs.grow(most);
+                most *= f;
+                up *= f;
+                xdelta *= f;
+                off *= f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[r] *= f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dq[i][r] *= f;
+            }
+            gs.top = fmaxf(gs.top, most);
+        }
         float t = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            dp[r] *= s[r];
-            t += dp[r];
-        }
+        for (int r = 0; r < 16; ++r) t += dp[r];
         off += t;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -968,9 +1053,13 @@ attn_dq_kernel(AttnArgs a) {
         if (it + 1 < turns) turn(it + 1, smem + kBuf, smem);
     }
     if (KG == 2) {
-        float* park = reinterpret_cast<float*>(smem) + (wave % W) * 64 * (NB * 32 + 1) + lane;
+        float* park = reinterpret_cast<float*>(smem) + (wave % W) * 64 * (NB * 32 + 3) + lane;
         if (grp == 1) {
             park[0] = off;
+            if (X::kScaled) {
+                park[64 * (NB * 32 + 1)] = gs.set() ? gs.x : INFINITY;
+                park[64 * (NB * 32 + 2)] = gs.top;
+            }
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -981,18 +1070,34 @@ attn_dq_kernel(AttnArgs a) {
         }
         __syncthreads();
         if (grp == 1) return;
-        off += park[0];
+        float f1 = 1.f, f2 = 1.f;
+        if (X::kScaled) {  // the smaller of the two factors (one that was not set goes with sums of 0)
+            const float x1 = gs.set() ? gs.x : INFINITY, x2 = park[64 * (NB * 32 + 1)], x = fminf(x1, x2);
+            if (x1 != INFINITY) f1 = x / x1;
+            if (x2 != INFINITY) f2 = x / x2;
+            if (x != INFINITY) gs.x = x, gs.limit = 32768.f;
+            gs.top = fmaxf(gs.top * f1, park[64 * (NB * 32 + 2)] * f2);
+        }
+        off = off * f1 + park[0] * f2;
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                dq[i][r] += park[64 * (1 + 32 * i + r)];
+                dq[i][r] = dq[i][r] * f1 + park[64 * (1 + 32 * i + r)] * f2;
                 pk[i][r] += park[64 * (17 + 32 * i + r)];
             }
     }
-    if (qi >= a.Tq) return;
     off = sum_halves(off);
-    if (hh == 0) a.delta[row] = delta + off;
+    const float unit = X::kScaled ? X::kUnprob / gs.x : 1.f;  // of dq and off
+    if (X::kScaled && q0 < a.Tq) {
+        // (the dK / dV kernel takes D corrected by off, which changes dS by off P at most)
+        float most = gs.set() && in ? (gs.top + fabsf(off)) / gs.x : 0.f;
+        if (!(most < INFINITY)) most = 0.f;  // a row whose gradient is not finite is no measure for the others
+        most = max_wave(most);
+        if (lane == 0) a.delta[delta_floats(a) + static_cast<long>(bh) * bounds_of_head(a) + (q0 >> 5)] = most;
+    }
+    if (qi >= a.Tq) return;
+    if (hh == 0) a.delta[row] = delta + off * unit;
     E* drow = static_cast<E*>(a.dq) + b * a.sdq.b + qi * a.sdq.t + h * a.sdq.h;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -1002,7 +1107,7 @@ attn_dq_kernel(AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
-                v[e] = static_cast<E>(in ? fmaf(-off, pk[i][r], dq[i][r]) * a.scale : 0.f);
+                v[e] = static_cast<E>(in ? fmaf(-off * X::kUnprob, pk[i][r], dq[i][r]) * (a.scale * unit) : 0.f);
             }
             const int c = 32 * i + 8 * g + 4 * hh;
             if (c < a.D) *reinterpret_cast<typename T::x4*>(drow + c) = v;
@@ -1019,6 +1124,7 @@ template <class E, int DP, bool kDrop, bool kFine>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 && !kFine ? 2 : 1)))
 attn_dkdv_kernel(AttnArgs a) {
     constexpr int R = kStage, NB = DP / 32;
+    typedef Exponent<E> X;
     typedef Tile<E, DP, R> T;
     typedef typename T::x8 x8;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1039,6 +1145,18 @@ attn_dkdv_kernel(AttnArgs a) {
     for (int i = 0; i < NB; ++i) { dk[i] = f32x16{0}; dv[i] = f32x16{0}; }
     const float sc2 = a.scale * kLog2e;
     const unsigned step = kDrop ? step_of(a) : 0u;
+    // half: dS times x, so that the bound of all queries that read this key head comes to [2^13, 2^14)
+    float x = X::kScaled ? 0.f : 1.f, xup = kDrop ? a.up : 1.f;
+    auto find_scale = [&]() {
+        const long nb = bounds_of_head(a), all = nb * group;  // (the heads of a group are neighbours)
+        const float* bounds = a.delta + delta_floats(a) + (static_cast<long>(b) * a.H + hk * group) * nb;
+        float most = 0.f;
+#pragma unroll 4
+        for (long i = lane; i < all; i += 64) most = fmaxf(most, bounds[i]);
+        most = max_wave(most);
+        x = most > 0.f ? ldexpf(1.f, min(14 - __builtin_amdgcn_frexp_expf(most), 60)) : 1.f;
+        xup *= x;
+    };
 
     constexpr int kBuf = 2 * T::kBytes + 2 * R * 4;
     typename T::Regs qr, dr;
@@ -1066,8 +1184,8 @@ attn_dkdv_kernel(AttnArgs a) {
             T::store(base, qr, tid);
             T::store(base + T::kBytes, dr, tid);
             if (tid < R) {
-                reinterpret_cast<float*>(base + 2 * T::kBytes)[tid] = ls == -INFINITY ? INFINITY : ls * kLog2e;
-                reinterpret_cast<float*>(base + 2 * T::kBytes)[R + tid] = de;
+                reinterpret_cast<float*>(base + 2 * T::kBytes)[tid] = ls == -INFINITY ? INFINITY : ls * kLog2e - X::kProb;
+                reinterpret_cast<float*>(base + 2 * T::kBytes)[R + tid] = X::kScaled ? de * x : de;
             }
         };
         auto tile = [&](const char* Qs, const char* Ds, const float* lse2, const float* del, int qs0) {
@@ -1121,7 +1239,9 @@ attn_dkdv_kernel(AttnArgs a) {
                     if (kDrop) {
                         const bool in = kept(w, r, a.limit);
                         pd[r] = in ? s[r] : 0.f;
-                        dp[r] = s[r] * fmaf(dp[r], in ? a.up : 0.f, -d4[e]);
+                        dp[r] = s[r] * fmaf(dp[r], in ? xup : 0.f, -d4[e]);
+                    } else if (X::kScaled) {
+                        dp[r] = s[r] * fmaf(dp[r], xup, -d4[e]);
                     } else {
                         dp[r] = s[r] * (dp[r] - d4[e]);
                     }
@@ -1163,6 +1283,7 @@ attn_dkdv_kernel(AttnArgs a) {
             __syncthreads();
         };
         fetch(lo);
+        if (X::kScaled && x == 0.f) find_scale();  // (once, while the first stage is on its way)
         fill(smem);
         __syncthreads();
         for (int st = lo; st < hi; st += 2) {
@@ -1172,7 +1293,8 @@ attn_dkdv_kernel(AttnArgs a) {
     }
     // register r of block i: key key0 + acc_row(r), column 32 i + n.  (The factor of what is kept
     // comes last: the probabilities are rounded without it, so that a probability of 1 stays exact.)
-    const float up = kDrop ? a.up : 1.f;
+    const float up = (kDrop ? a.up : 1.f) * X::kUnprob;
+    const float scale = X::kScaled ? a.scale * (X::kUnprob / (x > 0.f ? x : 1.f)) : a.scale;
     if (plan.ranges > 1) {
         const long heads = static_cast<long>(a.B) * a.Hk;
         float* pk = a.parts + ((2L * z * heads + bh) * a.Tk) * DP;
@@ -1183,7 +1305,7 @@ attn_dkdv_kernel(AttnArgs a) {
             if (j >= sq.n) continue;  // (not read)
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                pk[static_cast<long>(j) * DP + 32 * i + n] = dk[i][r] * a.scale;
+                pk[static_cast<long>(j) * DP + 32 * i + n] = dk[i][r] * scale;
                 pv[static_cast<long>(j) * DP + 32 * i + n] = dv[i][r] * up;
             }
         }
@@ -1200,7 +1322,7 @@ attn_dkdv_kernel(AttnArgs a) {
         for (int i = 0; i < NB; ++i) {
             const int c = 32 * i + n;
             if (c >= a.D) continue;
-            dkb[j * a.sdk.t + c] = static_cast<E>(in ? dk[i][r] * a.scale : 0.f);
+            dkb[j * a.sdk.t + c] = static_cast<E>(in ? dk[i][r] * scale : 0.f);
             dvb[j * a.sdv.t + c] = static_cast<E>(in ? dv[i][r] * up : 0.f);
         }
     }
@@ -1268,7 +1390,7 @@ int launch_fwd(const AttnArgs& a, hipStream_t s) {
 
 template <class E, int DP, bool kDrop, int KG, bool kFine>
 int launch_dq(const AttnArgs& a, hipStream_t s) {
-    constexpr int ring = 4 * KG * Tile<E, DP, kStage>::kBytes, park = KG == 2 ? 2 * 64 * (DP + 1) * 4 : 0;
+    constexpr int ring = 4 * KG * Tile<E, DP, kStage>::kBytes, park = KG == 2 ? 2 * 64 * (DP + 3) * 4 : 0;
     constexpr int lds = ring > park ? ring : park;
     if (const int st = set_lds(reinterpret_cast<const void*>(attn_dq_kernel<E, DP, kDrop, KG, kFine>), lds)) return st;
     hipLaunchKernelGGL((attn_dq_kernel<E, DP, kDrop, KG, kFine>), dim3(a.B * a.H, (a.Tq + 128 / KG - 1) / (128 / KG)),
@@ -1321,8 +1443,6 @@ int key_splits(const AttnArgs& a) {
     const long n = want < most ? want : most;
     return static_cast<int>(n < 1 ? 1 : n > 8 ? 8 : n);
 }
-long delta_floats(const AttnArgs& a) { return (static_cast<long>(a.B) * a.H * a.Tq + 3) & ~3L; }
-
 // Whether the backward pass undoes the rounding of P and dS: where there are so few pairs that the errors
 // do not average.  (Error of dQ over that of rounding alone: 1.0; without it 1.35 .. 1.7 at a few short
 // sequences, 1.41 .. 1.44 at many.  One sequence of 33: the same time; it would cost 32 sequences of 128,
@@ -1374,7 +1494,7 @@ long nf_attention_bwd_floats(const AttnArgs* args) {
     const AttnArgs& a = *args;
     if (a.Hk <= 0 || a.Tk <= 0) return 0;
     const int n = key_splits(a);
-    return delta_floats(a) + (n > 1 ? 2L * n * a.B * a.Hk * a.Tk * padded_dim(a.D) : 0);
+    return delta_floats(a) + bound_floats(a) + (n > 1 ? 2L * n * a.B * a.Hk * a.Tk * padded_dim(a.D) : 0);
 }
 
 // type: 1 bf16, 2 half.  backward 0: reads q, k, v and writes out, lse; 1: reads q, k, v, out,
@@ -1391,7 +1511,7 @@ int nf_attention(const AttnArgs* args, int type, int backward, hipStream_t s) {
         return -2;
     a.target = backward ? -1 : few_target(a);
     a.splits = backward ? key_splits(a) : 1;
-    if (backward) a.parts = a.delta + delta_floats(a);
+    if (backward) a.parts = a.delta + delta_floats(a) + bound_floats(a);
     if (type == 1) return a.D <= 64 ? launch<bf16, 64>(a, backward, s) : launch<bf16, 128>(a, backward, s);
     if (type == 2) return a.D <= 64 ? launch<half, 64>(a, backward, s) : launch<half, 128>(a, backward, s);
     return -1;

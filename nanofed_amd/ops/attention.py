@@ -302,8 +302,9 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     """Gradients of ``attention_fwd`` (called with the same arguments) from ``dout``: ``dq``, ``dk``,
     ``dv`` are written everywhere, with 0 behind the lengths.  The probabilities are computed again
     from ``lse`` and the mask from its counter; a key head's gradient is summed over the query heads
-    that share it in a fixed order, without atomics.  ``dq``, ``dk``, ``dv`` must not overlap what is
-    read."""
+    that share it in a fixed order, without atomics.  With float16 operands ``dout`` may be of any size
+    (no loss scaling is needed): the factors inside take the exponent that fits them.  ``dq``, ``dk``,
+    ``dv`` must not overlap what is read."""
     a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
     shape, shared, dtype, dev = q.shape, k.shape, q.dtype, q.device
     operands = (_operand(out, "out", shape, dtype, dev, False), _operand(dout, "dout", shape, dtype, dev, False),

@@ -1,0 +1,103 @@
+"""How far the gfx950 attention kernels are from the definition in 64 bits, in units of what rounding the
+exact result once leaves (root mean squares, so that no bound per element can hide a lost correction).
+
+Independent roundings add in squares: results whose operands P and dS were rounded to the same type are
+sqrt(2) = 1.42 times as far off as rounded results at most, so up to 1.5 is right for them."""
+
+import math
+
+import pytest
+import torch
+
+from nanofed_amd.ops import attention as A
+from tests import transformer_oracles as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, FP = torch.bfloat16, torch.float16
+TWO_ROUNDINGS = 1.5
+
+
+def rand(*shape, seed, dtype, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def inputs(B, Tq, Tk, H, Hk, D, dtype, dout=1.0, q=1.0, k=1.0):
+    return (rand(B, Tq, H, D, seed=1, dtype=dtype, scale=q), rand(B, Tk, Hk, D, seed=2, dtype=dtype, scale=k),
+            rand(B, Tk, Hk, D, seed=3, dtype=dtype), rand(B, Tq, H, D, seed=4, dtype=dtype, scale=dout))
+
+
+def run(q, k, v, dout=None, p=0.0, **how):
+    q, k, v = (t.to(DEV) for t in (q, k, v))
+    out, lse = A.attention_fwd(q, k, v, dropout=p, **how)
+    got = {"out": out}
+    if dout is not None:
+        got.update({n: torch.full_like(t, math.nan) for n, t in (("dq", q), ("dk", k), ("dv", v))})
+        A.attention_bwd(q, k, v, out, lse, dout.to(DEV), got["dq"], got["dk"], got["dv"], dropout=p, **how)
+    return got
+
+
+def off(got, want):
+    """Error over that of rounding the exact value once."""
+    want, got = want.double(), got.cpu()
+    rounded = (want.to(got.dtype).double() - want).square().mean().sqrt()
+    return float((got.double() - want).square().mean().sqrt() / rounded)
+
+
+def check(x, most, p=0.0, names=("dq", "dk", "dv"), **how):
+    want = oracle.attention(*x, p=p, **how)
+    got = run(*x, p=p, **how)
+    ratios = {n: round(off(got[n], want[n][0]), 3) for n in names}
+    assert all(r <= most for r in ratios.values()), ratios
+    return got
+
+
+# -- half has the exponents 2^-24 .. 2^15 only ------------------------------------------------------
+@pytest.mark.parametrize("dout", [1e2, 1.0, 1e-2, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("D,p", [(64, 0.0), (128, 0.1)])
+def test_half_gradients_of_any_size_against_many_keys(dout, D, p):
+    check(inputs(1, 2048, 2048, 2, 1, D, FP, dout=dout), TWO_ROUNDINGS, p=p, seed=3)
+
+
+@pytest.mark.parametrize("T", [33, 300])
+@pytest.mark.parametrize("dout", [1e2, 1e-4])
+def test_half_gradients_of_short_sequences(T, dout):
+    check(inputs(2, T, T, 2, 2, 64, FP, dout=dout), TWO_ROUNDINGS)
+
+
+def test_half_gradients_of_rows_of_different_sizes():
+    """Each query's gradient is as exact as if the others were not there."""
+    q, k, v, dout = inputs(1, 512, 512, 1, 1, 64, FP)
+    size = 10.0 ** torch.linspace(2, -4, 512)[torch.randperm(512, generator=torch.Generator().manual_seed(1))]
+    x = (q, k, v, (dout * size.view(1, -1, 1, 1)).to(FP))
+    want, got = oracle.attention(*x), run(*x)
+    for name in ("dq", "dk", "dv"):
+        assert off(got[name], want[name][0]) <= TWO_ROUNDINGS, name
+    small = size < 1e-2  # (their errors vanish in the mean of all rows)
+    assert off(got["dq"][:, small], want["dq"][0][:, small]) <= TWO_ROUNDINGS
+
+
+def test_half_gradients_whose_factors_pass_the_type_though_they_do_not():
+    """dS reaches 10^5, dQ and dK stay below 10^3."""
+    q, k, v, dout = inputs(1, 300, 300, 1, 1, 64, FP, dout=8e3, q=0.01, k=0.01)
+    got = check((q, k, v * 8, dout), TWO_ROUNDINGS)
+    assert all(bool(torch.isfinite(t).all()) for t in got.values())
+
+
+def test_half_value_gradients_of_small_probabilities():
+    """20000 keys: probabilities of 5e-5, below the smallest normal half."""
+    check(inputs(1, 256, 20000, 1, 1, 64, FP), TWO_ROUNDINGS, causal=False)
+
+
+def test_half_gradients_beside_a_row_that_is_not_finite():
+    """An infinite gradient of one query leaves the other queries' alone, and the keys behind its tile."""
+    q, k, v, dout = inputs(1, 200, 200, 1, 1, 64, FP, dout=1e-4)
+    want = oracle.attention(q, k, v, dout)
+    bad = dout.clone()
+    bad[0, 10] = math.inf
+    got = run(q, k, v, bad)
+    assert not bool(torch.isfinite(got["dq"][:, 10]).all())
+    rows = torch.arange(200) != 10
+    assert off(got["dq"][:, rows.to(DEV)], want["dq"][0][:, rows]) <= TWO_ROUNDINGS
+    for name in ("dk", "dv"):  # (query 10 sees keys 0 .. 10)
+        assert off(got[name][:, 64:], want[name][0][:, 64:]) <= TWO_ROUNDINGS, name

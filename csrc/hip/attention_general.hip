@@ -63,25 +63,28 @@ __device__ __forceinline__ halfx4 tr4(const half* p) {
 
 constexpr int kStage = 64;  // keys (or queries) per LDS stage
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// The reference that scores are taken relative to follows the running maximum only where that gets
-// ahead by a factor of 2^8 in the probability: any reference gives the same quotients, up to 2^8 fits
-// every type here with the same relative rounding, and what the sums so far would have to be
-// multiplied by at nearly every tile (some of 32 rows finds a new maximum) is spared.
-constexpr float kSlack = 8.f;
-
 // Half has the exponents 2^-14 .. 2^15 (2^-24 with fewer bits), and the factors P and dS = P (dP - D) of the
 // gradients leave them long before the gradients do: P is 1 / keys, dS that times dO.  So the backward
 // kernels hold P times 2^kProb, which a probability cannot carry beyond the type, and dS times a power of
 // two on top, which the dQ kernel finds for every query from what it meets (GradScale), the dK / dV kernel for
 // its workgroup from what the dQ kernel left (bounds).  Both are exact and are taken out in fp32.  bf16
 // has the exponents of fp32 and needs neither.
+//
+// In the forward pass the reference that scores are taken relative to follows the running maximum only
+// where that gets ahead by a factor of 2^kSlack in the probability: any reference gives the same quotients,
+// and what the sums so far would have to be multiplied by at nearly every tile (some of 32 rows finds a new
+// maximum) is spared.  bf16 has room for any slack.  In half what a probability is below the largest one
+// costs bits from 2^-14 on, and 2^22 keys of 2^-26 have 1 / 16 of the largest one's weight: there P carries
+// 2^kLift (so do the sums, which cancel it), and the slack is what is left of the type: 2^(3 + 12).
 template <class E> struct Exponent {
     static constexpr bool kScaled = false;
     static constexpr float kProb = 0.f, kUnprob = 1.f;  // 2^-kProb
+    static constexpr float kSlack = 8.f, kLift = 0.f;
 };
 template <> struct Exponent<half> {
     static constexpr bool kScaled = true;
     static constexpr float kProb = 15.f, kUnprob = 1.f / 32768.f;
+    static constexpr float kSlack = 3.f, kLift = 12.f;
 };
 
 struct Strides { long b, t, h; };  // elements between sequences, rows, heads
@@ -397,6 +400,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((DP ==
 attn_fwd_kernel(AttnArgs a) {
     typedef Tile<E, DP, kStage> T;
     typedef typename T::x8 x8;
+    typedef Exponent<E> X;
     constexpr int NB = DP / 32, W = 4 / KG, kQueries = 32 * W;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int bh = shifted_head(a, a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
@@ -448,12 +452,12 @@ attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
         for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
         mx = max_halves(mx);
-        if (__any((mx - m) * sc2 > kSlack)) {
+        if (__any((mx - m) * sc2 > X::kSlack)) {
             const float mn = fmaxf(m, mx);
             const float ref = mn == -INFINITY ? 0.f : mn;
             const float alpha = exp2_fast((m - ref) * sc2);
             m = mn;
-            msc = ref * sc2;
+            msc = ref * sc2 - X::kLift;
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
@@ -561,7 +565,7 @@ attn_fwd_kernel(AttnArgs a) {
             if (c < a.D) *reinterpret_cast<typename T::x4*>(orow + c) = v;
         }
     if (hh == 0)
-        a.lse[static_cast<long>(bh) * a.Tq + qi] = some ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+        a.lse[static_cast<long>(bh) * a.Tq + qi] = some ? m * a.scale + kLn2 * (__builtin_amdgcn_logf(l) - X::kLift) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -632,6 +636,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 
 attn_few_kernel(AttnArgs a) {
     typedef Tile<E, DP, 32> T;
     typedef typename T::x8 x8;
+    typedef Exponent<E> X;
     constexpr int NB = DP / 32, KS = DP / 16, kPer = 32 * T::kPieces / 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, n = lane & 31, hh = lane >> 5;
@@ -701,12 +706,12 @@ attn_few_kernel(AttnArgs a) {
             mx = fmaxf(mx, s[r]);
         }
         mx = max_halves(mx);
-        if (__any((mx - m) * sc2 > kSlack)) {
+        if (__any((mx - m) * sc2 > X::kSlack)) {
             const float mn = fmaxf(m, mx);
             const float ref = mn == -INFINITY ? 0.f : mn;
             const float alpha = exp2_fast((m - ref) * sc2);
             m = mn;
-            msc = ref * sc2;
+            msc = ref * sc2 - X::kLift;
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
@@ -791,7 +796,7 @@ attn_few_kernel(AttnArgs a) {
         }
         if (piece == 0)
             a.lse[(static_cast<long>(b) * a.H + head) * a.Tq + qr] =
-                some ? top * a.scale + kLn2 * __builtin_amdgcn_logf(sum) : -INFINITY;
+                some ? top * a.scale + kLn2 * (__builtin_amdgcn_logf(sum) - X::kLift) : -INFINITY;
     }
 }
 
@@ -862,7 +867,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
     if (DP > 64 && 64 + lane < a.D) orow[64 + lane] = static_cast<E>(some ? o1 * inv : 0.f);
     if (lane == 0)
         a.lse[(static_cast<long>(b) * a.H + h) * a.Tq + qi] =
-            some ? m * a.scale + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+            some ? m * a.scale + kLn2 * (__builtin_amdgcn_logf(l) - Exponent<E>::kLift) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -101,3 +101,21 @@ def test_half_gradients_beside_a_row_that_is_not_finite():
     assert off(got["dq"][:, rows.to(DEV)], want["dq"][0][:, rows]) <= TWO_ROUNDINGS
     for name in ("dk", "dv"):  # (query 10 sees keys 0 .. 10)
         assert off(got[name][:, 64:], want[name][0][:, 64:]) <= TWO_ROUNDINGS, name
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("Tq,D", [(40, 8), (1, 8), (40, 128)])
+def test_many_small_probabilities_behind_a_large_one(dtype, Tq, D):
+    """2^20 keys that each have e^-18 of the first one's weight have 1.6 % of it together."""
+    n, big = 1 << 20, 18.0
+    q, k = torch.zeros(1, Tq, 1, D, dtype=dtype, device=DEV), torch.zeros(1, n, 1, D, dtype=dtype, device=DEV)
+    v = torch.ones(1, n, 1, D, dtype=dtype, device=DEV)
+    q[..., 0], k[0, 0, 0, 0], v[0, 0] = 1.0, big, 0.0
+    out, lse = A.attention_fwd(q, k, v, scale=1.0, causal=False)
+    tail = (n - 1) * math.exp(-big)
+    # equal terms round alike: one rounding of P, one of the result, and 2^16 additions (16 keys each) in fp32
+    bound = 2 * oracle.UNIT[dtype] + 2.0**16 * 2.0**-24
+    assert float((out.double() / (tail / (1 + tail)) - 1).abs().max()) <= bound
+    # the sum of the probabilities is about 1 from the first key on, and each of 2^15 additions (32 keys) to it is
+    # off by up to 2^-24 of that, alike again
+    assert float((lse.double() - (big + math.log1p(tail))).abs().max()) <= big * 2.0**-22 + 2.0**15 * 2.0**-24 * (1 + tail)

@@ -631,8 +631,13 @@ __device__ __forceinline__ Chunk few_chunk(const AttnArgs& a, int id, int lane) 
     return {-1, 0, 0, 0, 0, {0, 0, 0}};
 }
 
-template <class E, int DP, bool kFine>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 128 && kFine ? 1 : 2)))
+//
+// kTwice: up to 16 rows (queries times heads that share a key head), so the tile's other 16 columns are
+// free, and they undo the rounding of P: they hold the same rows again, as P less what the first ones round
+// it to, and the joint adds them.  It costs the subtraction only, no product and no read.  (Error of one head
+// of 64 against 680 keys over that of rounding the output: 1.0, without it 1.3 .. 1.5.)
+template <class E, int DP, bool kTwice>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 attn_few_kernel(AttnArgs a) {
     typedef Tile<E, DP, 32> T;
     typedef typename T::x8 x8;
@@ -646,8 +651,10 @@ attn_few_kernel(AttnArgs a) {
     const int b = me.b, hk = me.hk, group = a.H / a.Hk;
     const Seq sq = me.seq;
     const int row0 = 32 * blockIdx.y, all = a.Tq * group, rows = min(32, all - row0);  // of this tile
-    const int qi = (row0 + n) / group, h = hk * group + (row0 + n) % group;
-    const bool in = n < rows && qi < sq.m;
+    const int own = kTwice ? n & 15 : n;  // row of the tile that this column has
+    const int qi = (row0 + own) / group, h = hk * group + (row0 + own) % group;
+    const bool in = own < rows && qi < sq.m;
+    const float second = n < 16 ? 0.f : 1.f;
     const int seen = (in ? keys_seen(sq, qi) : 0) - 4 * hh;
     const int k0 = me.at * me.size, k1 = min(sq.m > 0 ? sq.n : 0, k0 + me.size);
     char* lds = smem + wave * 2 * T::kBytes;  // K, V
@@ -725,19 +732,15 @@ attn_few_kernel(AttnArgs a) {
             rs += s[r];
         }
         l += rs;
+        if (kTwice) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(static_cast<float>(static_cast<E>(s[r])), -second, s[r]);
+        }
         const x8 p0 = pack8<E>(s, 0), p1 = pack8<E>(s, 8);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             o[i] = mma(T::tr(lds + T::kBytes, at, 0, i), p0, o[i]);
             o[i] = mma(T::tr(lds + T::kBytes, at, 16, i), p1, o[i]);
-        }
-        if (kFine) {  // what the rounding of P leaves
-            const x8 r0 = rest8<E>(s, 0), r1 = rest8<E>(s, 8);
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                o[i] = mma(T::tr(lds + T::kBytes, at, 0, i), r0, o[i]);
-                o[i] = mma(T::tr(lds + T::kBytes, at, 16, i), r1, o[i]);
-            }
         }
     }
     l = sum_halves(l);
@@ -750,7 +753,7 @@ attn_few_kernel(AttnArgs a) {
         ml[wave * 64 + 32 + n] = l;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (n < rows) {
+    if (own < rows) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -774,10 +777,14 @@ attn_few_kernel(AttnArgs a) {
         for (int w = 0; w < 4; ++w) {
             const float f = exp2_fast((mw[w] - ref) * sc2);
             sum = fmaf(ml[w * 64 + 32 + row], f, sum);
-            const f32x4 part = *reinterpret_cast<const f32x4*>(
-                smem + w * 2 * T::kBytes + (row * kPieces + (piece ^ (row & (kPieces - 1)))) * 16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], f, v[e]);
+            for (int again = 0; again < (kTwice ? 32 : 16); again += 16) {
+                const int at = row + again;
+                const f32x4 part = *reinterpret_cast<const f32x4*>(
+                    smem + w * 2 * T::kBytes + (at * kPieces + (piece ^ (at & (kPieces - 1)))) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], f, v[e]);
+            }
         }
         if (me.count > 1) {
             const long part = static_cast<long>(blockIdx.x) * all + row0 + row;
@@ -886,8 +893,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
 // 244 us), and a workgroup's time is 9 us + 1.2 us per 32 keys, which is what bounds ragged batches.
 //
 // kFine: P and dS are rounded to the operands' type for the products, an error like that of rounding
-// the results, so that the two add up to sqrt(2) of one over many terms.  Over few a sum can come out
-// worse; then the rounding is undone by a product with what it left (see fine).
+// the results, so that the two add up to sqrt(2) of one.  Short sequences undo it by a product with what
+// the rounding left (see fine).
 template <class E, int DP, bool kDrop, int KG, bool kFine>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 ? 2 : 1)))
 attn_dq_kernel(AttnArgs a) {
@@ -1421,17 +1428,12 @@ int few_target(const AttnArgs& a) {
 int few_workgroups(const AttnArgs& a) { return a.target + a.B * a.Hk; }  // at most
 int padded_dim(int D) { return D <= 64 ? 64 : 128; }
 
-// Whether few queries undo the rounding of P: where there are so few outputs that their errors do not
-// average (one head of 64 against 680 keys: 1.3 .. 1.5 times that of rounding the output, 1.0 undone).
-// It costs 11 % where the keys are read at full rate (four caches of up to 8191 keys: 25.2 -> 28.0 us).
-bool few_outputs(const AttnArgs& a) { return static_cast<long>(a.B) * a.H * a.Tq * a.D <= 4096; }
-
-template <class E, int DP, bool kFine>
+template <class E, int DP, bool kTwice>
 int launch_few(const AttnArgs& a, hipStream_t s) {
     constexpr int lds = 8 * Tile<E, DP, 32>::kBytes + 4 * 64 * 4;
     if (a.target != 0 && a.parts == nullptr) return -2;
-    if (const int st = set_lds(reinterpret_cast<const void*>(attn_few_kernel<E, DP, kFine>), lds)) return st;
-    hipLaunchKernelGGL((attn_few_kernel<E, DP, kFine>), dim3(few_workgroups(a), few_tiles(a)), dim3(256), lds, s, a);
+    if (const int st = set_lds(reinterpret_cast<const void*>(attn_few_kernel<E, DP, kTwice>), lds)) return st;
+    hipLaunchKernelGGL((attn_few_kernel<E, DP, kTwice>), dim3(few_workgroups(a), few_tiles(a)), dim3(256), lds, s, a);
     if (a.target != 0)
         hipLaunchKernelGGL((attn_join_kernel<E, DP>), dim3((a.B * a.H * a.Tq + 3) / 4), dim3(256), 0, s, a,
                            few_workgroups(a));
@@ -1448,11 +1450,12 @@ int key_splits(const AttnArgs& a) {
     const long n = want < most ? want : most;
     return static_cast<int>(n < 1 ? 1 : n > 8 ? 8 : n);
 }
-// Whether the backward pass undoes the rounding of P and dS: where there are so few pairs that the errors
-// do not average.  (Error of dQ over that of rounding alone: 1.0; without it 1.35 .. 1.7 at a few short
-// sequences, 1.41 .. 1.44 at many.  One sequence of 33: the same time; it would cost 32 sequences of 128,
-// 12 heads of 64, 28 -> 37 us.)
-bool fine(const AttnArgs& a) { return static_cast<double>(a.B) * a.H * a.Tq * a.Tk <= 524288.0; }
+// Whether the backward pass undoes the rounding of P and dS: for short sequences (by the lengths of the call
+// alone, so that a sequence has the same gradients whatever shares its launch).  Error of dQ and dK over that of
+// rounding them: 1.0, without it 1.41 at any length.  It costs nothing where launches bound the time (8
+// sequences of 64, 12 heads of 64: 18.5 us both ways) and up to half where they are many (256 of them: 88 -> 128
+// us; 30 % for 128 sequences of 128 or 8 of 1024, where attention is more of a layer's time).
+bool fine(const AttnArgs& a) { return a.Tq <= kStage && a.Tk <= kStage; }
 
 template <class E, int DP, bool kDrop, bool kFine>
 int launch_bwd(const AttnArgs& a, hipStream_t s) {
@@ -1471,7 +1474,7 @@ template <class E, int DP>
 int launch(const AttnArgs& a, int backward, hipStream_t s) {
     if (backward && fine(a)) return a.limit ? launch_bwd<E, DP, true, true>(a, s) : launch_bwd<E, DP, false, true>(a, s);
     if (backward) return a.limit ? launch_bwd<E, DP, true, false>(a, s) : launch_bwd<E, DP, false, false>(a, s);
-    if (a.target >= 0) return few_outputs(a) ? launch_few<E, DP, true>(a, s) : launch_few<E, DP, false>(a, s);
+    if (a.target >= 0) return a.Tq * (a.H / a.Hk) <= 16 ? launch_few<E, DP, true>(a, s) : launch_few<E, DP, false>(a, s);
     if (halve_keys(a)) return a.limit ? launch_fwd<E, DP, true, 2>(a, s) : launch_fwd<E, DP, false, 2>(a, s);
     return a.limit ? launch_fwd<E, DP, true, 1>(a, s) : launch_fwd<E, DP, false, 1>(a, s);
 }

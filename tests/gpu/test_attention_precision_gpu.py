@@ -119,3 +119,58 @@ def test_many_small_probabilities_behind_a_large_one(dtype, Tq, D):
     # the sum of the probabilities is about 1 from the first key on, and each of 2^15 additions (32 keys) to it is
     # off by up to 2^-24 of that, alike again
     assert float((lse.double() - (big + math.log1p(tail))).abs().max()) <= big * 2.0**-22 + 2.0**15 * 2.0**-24 * (1 + tail)
+
+
+# -- which roundings are undone ---------------------------------------------------------------------
+ONE_ROUNDING = 1.1  # (sums in fp32 and what is left of the two roundings come on top)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("B,T,H,Hk,D", [(1, 64, 1, 1, 64), (2, 33, 2, 2, 128), (40, 64, 12, 12, 64), (300, 9, 8, 2, 64)])
+@pytest.mark.parametrize("p", [0.0, 0.2])
+def test_gradients_of_short_sequences_are_off_by_one_rounding(dtype, B, T, H, Hk, D, p):
+    check(inputs(B, T, T, H, Hk, D, dtype), ONE_ROUNDING, p=p, seed=4)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("B,T,H,Hk,D", [(1, 65, 2, 2, 64), (2, 129, 4, 1, 64), (1, 700, 1, 1, 64), (3, 300, 2, 2, 128)])
+def test_longer_sequences_are_off_by_two_roundings(dtype, B, T, H, Hk, D):
+    check(inputs(B, T, T, H, Hk, D, dtype), TWO_ROUNDINGS, names=("out", "dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (FP, 64), (BF, 128)])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk", [(1, 1, 700, 1, 1), (1, 1, 77, 4, 4), (9, 2, 2050, 8, 1), (3, 4, 900, 8, 2), (2, 16, 300, 3, 3)])
+def test_up_to_16_rows_that_share_keys_are_off_by_one_rounding(dtype, D, B, Tq, Tk, H, Hk):
+    check(inputs(B, Tq, Tk, H, Hk, D, dtype)[:3], ONE_ROUNDING, names=("out",))
+
+
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk", [(2, 17, 700, 4, 4), (2, 5, 1500, 8, 1), (2, 32, 1024, 4, 2)])
+def test_more_rows_are_off_by_two_roundings(B, Tq, Tk, H, Hk):
+    check(inputs(B, Tq, Tk, H, Hk, 64, BF)[:3], TWO_ROUNDINGS, names=("out",))
+
+
+@pytest.mark.parametrize("T,most", [(64, ONE_ROUNDING), (200, TWO_ROUNDINGS)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_gradients_where_the_rounding_of_the_output_counts(T, most, dtype):
+    """Values with a common offset make an output whose rounding, were D = rowsum(dO * O) left as it is, would
+    outweigh the other two."""
+    q, k, v, dout = inputs(1, T, T, 2, 2, 64, dtype)
+    check((q, k, (v.float() + 64).to(dtype), dout), most, names=("dq", "dk"))
+
+
+@pytest.mark.parametrize("T", [7, 64, 128])
+def test_a_sequence_has_the_same_bits_whatever_shares_its_launch(T):
+    B, H, D = 96, 12, 64
+    x = [t.to(DEV) for t in inputs(B, T, T, H, H, D, BF)]
+    whole = run(*x[:3], x[3], p=0.1, seed=3, step=2)
+    for b in (0, 41, 95):
+        alone = run(*(t[b:b + 1] for t in x[:3]), x[3][b:b + 1], p=0.1, seed=3, step=2, first_batch=b)
+        assert all(torch.equal(alone[n][0], whole[n][b]) for n in whole), b
+
+
+def test_a_token_has_the_same_bits_whatever_shares_its_launch():
+    B, Tk, H, D = 96, 120, 12, 64
+    q, k, v, _ = (t.to(DEV) for t in inputs(B, 1, Tk, H, H, D, BF))
+    whole = run(q, k, v)["out"]
+    for b in (0, 41, 95):
+        assert torch.equal(run(q[b:b + 1], k[b:b + 1], v[b:b + 1])["out"][0], whole[b]), b

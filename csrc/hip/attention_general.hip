@@ -582,7 +582,7 @@ attn_fwd_kernel(AttnArgs a) {
 // 19.0 us + 5.4 us for the join with 512 workgroups, 4.4 TB/s; 23.0 + 4.9 with 256; without the
 // hint that the keys are read once, which leaves the parts in L2, 20.2 + 6.2.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-constexpr int kFewQueries = 32, kFewRows = 256, kFewMaxBatch = 512, kFewTarget = 512;
+constexpr int kFewQueries = 32, kFewRows = 256, kFewTarget = 512;
 constexpr int kOnce = 2;  // non-temporal load
 
 struct Chunk { int b, hk, count, at, size; Seq seq; };  // chunk `at` of `count` of (b, hk), keys per chunk
@@ -607,7 +607,7 @@ __device__ __forceinline__ Chunk few_chunk(const AttnArgs& a, int id, int lane) 
     const Seq mine0 = lane < a.B ? sequence(a, lane) : Seq{0, 0, 0};
     long keys = few_keys(mine0);
     for (int i = lane + 64; i < a.B; i += 64) keys += few_keys(sequence(a, i));
-    const int size = few_size(a, lane_sum(static_cast<int>(keys)));
+    const int size = few_size(a, lane_sum(static_cast<int>(keys)));  // (fewer than 512 sequences of up to 2^22)
     int before = 0;  // parts of the sequences before
     for (int i0 = 0; i0 < a.B; i0 += 64) {
         const Seq mine = i0 == 0 ? mine0 : (i0 + lane < a.B ? sequence(a, i0 + lane) : Seq{0, 0, 0});
@@ -1423,7 +1423,7 @@ int few_target(const AttnArgs& a) {
     if (a.limit != 0 || a.Tq > kFewQueries || group > kFewRows || a.Tq * group > kFewRows) return -1;
     const int tiles = few_tiles(a), target = kFewTarget / tiles;
     if (tiles > 1 && (a.Tk < 1024 || (2 * tiles > group && static_cast<long>(a.B) * a.H > 128))) return -1;
-    return a.B <= kFewMaxBatch && static_cast<long>(a.B) * a.Hk < target && a.Tk > 128 ? target : 0;
+    return static_cast<long>(a.B) * a.Hk < target && a.Tk > 128 ? target : 0;
 }
 int few_workgroups(const AttnArgs& a) { return a.target + a.B * a.Hk; }  // at most
 int padded_dim(int D) { return D <= 64 ? 64 : 128; }

@@ -277,6 +277,7 @@ class GPT2NativeTrainer(GroupTrainer):
             return
         embed_ops.embedding_bwd(tokens.view(batch, seq), dx, g["wte.weight"], dpositions=g["wpe.weight"],
                                 accumulate=True, dropout=masks.embd,
+                                order=(order[0], order[1]) if order is not None else None,
                                 **masks.rows(seq, dx.shape[-1], "embd", client=client))
 
     def _attn_args(self, l: int, qkv: torch.Tensor, b: _Buffers, masks: _Masks | None):
@@ -509,8 +510,8 @@ class GPT2NativeTrainer(GroupTrainer):
     def _gstep(self, g0: int, Gn: int, tokens: torch.Tensor,
                order: torch.Tensor | None = None, number: "int | torch.Tensor" = 0) -> None:
         """One optimisation step of Gn clients; ``tokens`` ``[Gn * batch, seq + 1]``,
-        client-major.  ``order`` ``[Gn, 2, batch * seq]``: per client the sorted input tokens
-        and their stable sort order (drawn on the host with the batch); without it the
+        client-major.  ``order`` ``[Gn, 2, batch * seq]`` (``_order_type``): per client the sorted input
+        tokens and their stable sort order (drawn on the host with the batch); without it the
         embedding gradient sorts on the device.  ``number``: the step's number for the dropout
         masks, or one int64 on the device that holds it."""
         cfg, m, L = self.cfg, self.m, self.m.n_layer
@@ -627,8 +628,8 @@ class GPT2NativeTrainer(GroupTrainer):
         the embedding gradient) are assembled on the host for the whole round - the host
         holds a copy of the token shard and draws the shuffles itself - and copied into the
         graph's static input buffers before each replay; the captured step holds no sort,
-        no gather and no allocation (with embedding dropout it holds the sort and the scratch
-        memory of that operator's gradient).  The first step of a (first client, group size) pair
+        no gather and no allocation (with dropout it holds the scratch memory of the embedding's
+        and the attention's gradients).  The first step of a (first client, group size) pair
         runs eagerly on the same buffers (it warms the workspaces up), the second is
         captured, every later one is a replay."""
         cfg = self.cfg
@@ -640,7 +641,7 @@ class GPT2NativeTrainer(GroupTrainer):
         E = cfg.local_epochs
         # the round's batches, in page-locked memory: [epoch, step, client] blocks
         tok = torch.empty(E, steps, G * B, S1, dtype=torch.int64).pin_memory()
-        order = torch.empty(E, steps, G, 2, B * (S1 - 1), dtype=torch.int64).pin_memory()
+        order = torch.empty(E, steps, G, 2, B * (S1 - 1), dtype=self._order_type()).pin_memory()
         number = torch.tensor([[self._step_number(round_idx, e, s) for s in range(steps)]
                                for e in range(E)], dtype=torch.int64).pin_memory()
         for epoch in range(E):
@@ -675,13 +676,17 @@ class GPT2NativeTrainer(GroupTrainer):
                         self._gstep(g0, Gn, st["tokens"], st["order"], st["number"])
                         st["warm"] = True
 
+    def _order_type(self) -> torch.dtype:
+        """Of the sorted tokens and their order, as the embedding's gradient takes them."""
+        return torch.int32 if self.m.embd_dropout else torch.int64
+
     def _static_inputs(self, g0: int, Gn: int, S1: int) -> dict:
         key = (g0, Gn)
         if key not in self._step_inputs:
             B = self.cfg.batch_size
             self._step_inputs[key] = {
                 "tokens": torch.zeros(Gn * B, S1, dtype=torch.int64, device=self.device),
-                "order": torch.zeros(Gn, 2, B * (S1 - 1), dtype=torch.int64, device=self.device),
+                "order": torch.zeros(Gn, 2, B * (S1 - 1), dtype=self._order_type(), device=self.device),
                 "number": torch.zeros((), dtype=torch.int64, device=self.device),
                 "warm": False,
             }

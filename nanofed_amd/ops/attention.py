@@ -26,7 +26,7 @@ import torch.nn.functional as F
 from nanofed_amd.core.exceptions import DeviceError
 
 from . import library
-from .dropout import check_key, limit_of, philox_words
+from .dropout import check_key, limit_of, philox_words, refuse_recording
 
 P, I, L = c_void_p, c_int, c_long
 _SIGS = {
@@ -256,7 +256,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     ``j <= i + keys - queries`` (equal numbers: the usual triangle; one query: all of the cache).
     Queries behind the length and queries that see no key give 0 and a log-sum-exp of -inf.  A
     non-finite value that some query sees may spread to other queries of its sequence.  ``out`` and
-    ``lse`` must not overlap what is read.
+    ``lse`` must not overlap what is read.  Not recorded by autograd: a tensor that requires a gradient
+    is refused while gradients are enabled.
 
     ``dropout`` (taken to a multiple of 1 / 256): each probability is dropped with it, what stays is
     scaled by the inverse of the share that stays.  The mask is a function of ``seed``, ``step`` (a
@@ -264,6 +265,7 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     query and key: probability (i, j) of head h of sequence b takes byte ``j & 3`` of word ``i & 3`` of
     the Philox4x32-7 block with counter ``(j >> 2, i >> 2, (first_batch + b) H + h, step)``."""
     a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
+    refuse_recording("attention", q, k, v, out, lse)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if lse is None:
@@ -306,6 +308,7 @@ def attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     (no loss scaling is needed): the factors inside take the exponent that fits them.  ``dq``, ``dk``,
     ``dv`` must not overlap what is read."""
     a = _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step, first_batch)
+    refuse_recording("attention", q, k, v, out, lse, dout, dq, dk, dv)
     shape, shared, dtype, dev = q.shape, k.shape, q.dtype, q.device
     operands = (_operand(out, "out", shape, dtype, dev, False), _operand(dout, "dout", shape, dtype, dev, False),
                 _operand(dq, "dq", shape, dtype, dev, True), _operand(dk, "dk", shared, dtype, dev, True),

@@ -82,6 +82,14 @@ def step_args(step: "int | torch.Tensor") -> tuple[int, int]:
     return 0, step
 
 
+def refuse_recording(what: str, *tensors: "torch.Tensor | None") -> None:
+    """Raises for a tensor that autograd would follow: the kernels' results are not recorded, so its
+    gradient would be lost without a word."""
+    if any(t is not None and t.requires_grad for t in tensors) and torch.is_grad_enabled():
+        raise DeviceError(f"{what}: autograd does not record this operator: call it under torch.no_grad() (its "
+                          "gradient is an operator of its own), or give it detached tensors")
+
+
 def check_first(first: int, what: str) -> None:
     if not 0 <= first < 1 << 62:
         raise DeviceError(f"{what}: first must not be negative (nor pass 2^62)")
@@ -123,12 +131,14 @@ def dropout_fwd(x: torch.Tensor, p: float, *, seed: int, step: "int | torch.Tens
     are those of the contiguous tensor).  ``out`` may be ``x`` or ``residual``; without it a
     contiguous tensor is made.  ``step``: a number, or one int64 on the device that the kernel
     reads when it runs.  ``first``: the place of the first element, so that a tensor can be done
-    in parts."""
+    in parts.  Not recorded by autograd (a tensor that requires a gradient is refused while gradients
+    are enabled)."""
     limit = limit_of(p, 16, "dropout")
     if x.dtype not in FLOAT_TYPES:
         raise DeviceError(f"dropout: float32, bfloat16 or float16, got {x.dtype}")
     check_first(first, "dropout")
     check_key(seed, step, x.device, "dropout")
+    refuse_recording("dropout", x, residual, out)
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     for t, name in ((residual, "residual"), (out, "out")):

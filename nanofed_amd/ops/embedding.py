@@ -24,7 +24,7 @@ import torch
 from nanofed_amd.core.exceptions import DeviceError
 
 from . import library
-from .dropout import FLOAT_TYPES, check_first, check_key, kept_rows, limit_of, step_args
+from .dropout import FLOAT_TYPES, check_first, check_key, kept_rows, limit_of, refuse_recording, step_args
 
 P, L, I, ARGS = c_void_p, c_long, c_int, c_char_p
 _SIGS = {
@@ -82,7 +82,7 @@ def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor |
                   seed: int = 0, step: "int | torch.Tensor" = 0, first: int = 0) -> torch.Tensor:
     """``drop(scale * table[tokens] + positions[t])`` for ``tokens`` ``[T]`` or ``[B, T]``;
     ``positions`` (optional) has at least T rows.  ``dropout``, ``seed``, ``step``, ``first``: as
-    in ``ops.dropout``."""
+    in ``ops.dropout``.  Not recorded by autograd."""
     if table.dim() != 2 or table.dtype not in FLOAT_TYPES or not table.is_contiguous():
         raise DeviceError("embedding: the table must be a contiguous float matrix")
     dev, (V, C) = table.device, table.shape
@@ -90,6 +90,7 @@ def embedding_fwd(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor |
     limit = limit_of(dropout, 16, "embedding")
     check_key(seed, step, dev, "embedding")
     check_first(first, "embedding")
+    refuse_recording("embedding", table, positions, out)
     if positions is not None:
         if positions.dim() != 2 or positions.shape[0] < T:
             raise DeviceError(f"embedding: positions must have at least {T} rows")
@@ -179,6 +180,7 @@ def embedding_bwd(tokens: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor
     limit = limit_of(dropout, 16, "embedding")
     check_key(seed, step, dev, "embedding")
     check_first(first, "embedding")
+    refuse_recording("embedding", dout, dtable, dpositions)
     if dout.numel() != R * C or (dout.numel() and dout.shape[-1] != C) or not dout.is_contiguous():
         raise DeviceError(f"embedding: dout must be {R} contiguous rows of {C}")
     _need(dtable, (V, C), (dout.dtype, torch.float32), dev, "dtable")

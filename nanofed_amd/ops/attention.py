@@ -259,8 +259,8 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     ``lse`` must not overlap what is read.  Not recorded by autograd: a tensor that requires a gradient
     is refused while gradients are enabled.
 
-    ``dropout`` (taken to a multiple of 1 / 256): each probability is dropped with it, what stays is
-    scaled by the inverse of the share that stays.  The mask is a function of ``seed``, ``step`` (a
+    ``dropout`` (taken to a multiple of 1 / 256: 0.1 is 0.1016; less than 1 / 512 is refused): each
+    probability is dropped with it, what stays is scaled by the inverse of the share that stays.  The mask is a function of ``seed``, ``step`` (a
     number, or one int64 on the device that the kernel reads when it runs) and of the sequence, head,
     query and key: probability (i, j) of head h of sequence b takes byte ``j & 3`` of word ``i & 3`` of
     the Philox4x32-7 block with counter ``(j >> 2, i >> 2, (first_batch + b) H + h, step)``."""

@@ -57,11 +57,14 @@ def site_seed(seed: int, *site) -> int:
 
 # -- the generator ------------------------------------------------------------------------
 def limit_of(p: float, bits: int, what: str) -> int:
-    """The threshold ``round(2^bits p)`` of a dropout probability."""
+    """The threshold ``round(2^bits p)`` of a dropout probability; one that is not 0 but would be taken
+    to 0 is refused."""
     limit = round(p * (1 << bits)) if 0.0 <= p < 1.0 else 1 << bits
     if limit >= 1 << bits:
         raise DeviceError(f"{what}: the dropout probability must be in [0, 1) and round below 1 "
                           f"at {bits} bits, got {p}")
+    if limit == 0 and p > 0.0:
+        raise DeviceError(f"{what}: the dropout probability is taken to a multiple of 2^-{bits}, {p} would drop nothing")
     return limit
 
 

@@ -7,6 +7,7 @@ from nanofed_amd.core.exceptions import DeviceError
 from nanofed_amd.ops import attention as A
 from nanofed_amd.ops import dropout as D
 from nanofed_amd.ops import embedding as E
+from tests.unit.test_gpt2_dropout_cpu import _engine
 
 
 def test_tensors_that_autograd_would_follow_are_refused():
@@ -28,3 +29,20 @@ def test_tensors_that_autograd_would_follow_are_refused():
             call()
         with torch.no_grad():
             call()
+
+
+def test_a_dropout_that_would_drop_nothing_is_refused():
+    q, x, tok = torch.zeros(1, 4, 2, 8), torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    for p in (0.0019, 1e-9):
+        with pytest.raises(DeviceError, match="would drop nothing"):
+            A.attention_fwd(q, q, q, dropout=p)
+    for call in (lambda p: D.dropout_fwd(x, p, seed=1), lambda p: E.embedding_fwd(tok, x, dropout=p),
+                 lambda p: E.embedding_bwd(tok, x, x.clone(), dropout=p)):
+        with pytest.raises(DeviceError, match="would drop nothing"):
+            call(7e-6)
+        call(8e-6)
+        call(0.0)
+    A.attention_fwd(q, q, q, dropout=0.002)
+    with pytest.raises(DeviceError, match="would drop nothing"):
+        _engine(dict(dropout=0.001))
+    _engine(dict(resid_dropout=0.001))

@@ -219,8 +219,8 @@ def _arguments(q, k, v, causal, scale, q_lengths, k_lengths, dropout, seed, step
     check_key(seed, step, dev, "attention")
     a.seed = seed
     a.step_at, a.step = (step.data_ptr(), 0) if isinstance(step, torch.Tensor) else (0, step)
-    if not 0 <= first_batch < 1 << 32:
-        raise DeviceError("attention: first_batch must not be negative (nor pass 2^32)")
+    if not 0 <= first_batch or (first_batch + B) * H > 1 << 32:
+        raise DeviceError("attention: first_batch must not be negative, nor (first_batch + batch) * heads pass 2^32")
     a.first_head = first_batch * H
     a.causal = bool(causal)
     shared = (B, Tk, Hk, D)

@@ -46,3 +46,13 @@ def test_a_dropout_that_would_drop_nothing_is_refused():
     with pytest.raises(DeviceError, match="would drop nothing"):
         _engine(dict(dropout=0.001))
     _engine(dict(resid_dropout=0.001))
+
+
+def test_masks_that_would_repeat_are_refused():
+    """The sequence and head are 32 bits of the mask's counter."""
+    q = torch.zeros(2, 4, 4, 8)
+    how = dict(dropout=0.5, seed=1)
+    A.attention_fwd(q, q, q, first_batch=(1 << 30) - 2, **how)
+    for first in ((1 << 30) - 1, 1 << 30, (1 << 32) - 1):
+        with pytest.raises(DeviceError, match="first_batch"):
+            A.attention_fwd(q, q, q, first_batch=first, **how)

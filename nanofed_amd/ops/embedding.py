@@ -191,12 +191,14 @@ def embedding_bwd(tokens: torch.Tensor, dout: torch.Tensor, dtable: torch.Tensor
     if order is not None:
         for t, name in zip(order, ("key", "order")):
             _need(t, (R,), (torch.int32,), dev, name)
-    if R == 0 or C == 0 or V == 0:
+    if R == 0 or C == 0:
         if not accumulate:
             dtable.zero_()
-        if dpositions is not None and R == 0:
+        if dpositions is not None:
             dpositions[:T].zero_()
         return
+    if V == 0:
+        raise DeviceError("embedding: the table has no rows")
     if dev.type != "cuda":
         d = dout.reshape(B, T, C).float()
         if limit:

@@ -56,3 +56,14 @@ def test_masks_that_would_repeat_are_refused():
     for first in ((1 << 30) - 1, 1 << 30, (1 << 32) - 1):
         with pytest.raises(DeviceError, match="first_batch"):
             A.attention_fwd(q, q, q, first_batch=first, **how)
+
+
+def test_tokens_of_a_table_without_rows_are_refused_both_ways():
+    """(the gradient left that of the positions as it was)"""
+    tok, none, pos = torch.zeros(2, 3, dtype=torch.int64), torch.zeros(0, 4), torch.full((3, 4), 7.0)
+    with pytest.raises(DeviceError, match="no rows"):
+        E.embedding_fwd(tok, none)
+    with pytest.raises(DeviceError, match="no rows"):
+        E.embedding_bwd(tok, torch.ones(2, 3, 4), none, dpositions=pos)
+    E.embedding_bwd(tok[:0], torch.ones(0, 3, 4), none, dpositions=pos)
+    assert bool((pos == 0).all())

@@ -88,9 +88,12 @@ def step_args(step: "int | torch.Tensor") -> tuple[int, int]:
 def refuse_recording(what: str, *tensors: "torch.Tensor | None") -> None:
     """Raises for a tensor that autograd would follow: the kernels' results are not recorded, so its
     gradient would be lost without a word."""
-    if any(t is not None and t.requires_grad for t in tensors) and torch.is_grad_enabled():
-        raise DeviceError(f"{what}: autograd does not record this operator: call it under torch.no_grad() (its "
-                          "gradient is an operator of its own), or give it detached tensors")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise DeviceError(f"{what}: autograd does not record this operator: call it under torch.no_grad() (its "
+                              "gradient is an operator of its own), or give it detached tensors")
 
 
 def check_first(first: int, what: str) -> None:

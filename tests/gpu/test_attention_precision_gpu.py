@@ -174,3 +174,60 @@ def test_a_token_has_the_same_bits_whatever_shares_its_launch():
     whole = run(q, k, v)["out"]
     for b in (0, 41, 95):
         assert torch.equal(run(q[b:b + 1], k[b:b + 1], v[b:b + 1])["out"][0], whole[b]), b
+
+
+# -- half: what the factors must not depend on --------------------------------------------------------
+@pytest.mark.parametrize("Tq,Tk,D,p", [(90, 90, 64, 0.2), (300, 300, 128, 0.0), (64, 50, 64, 0.0), (600, 200, 64, 0.1)])
+def test_half_gradients_do_not_depend_on_what_lies_behind_the_lengths(Tq, Tk, D, p):
+    q, k, v, dout = inputs(3, Tq, Tk, 2, 1, D, FP, dout=1e-3)
+    nq, nk = [Tq // 2, 0, Tq], [Tk // 2, 0, Tk]
+    how = dict(q_lengths=torch.tensor(nq, dtype=torch.int32, device=DEV),
+               k_lengths=torch.tensor(nk, dtype=torch.int32, device=DEV), p=p, seed=6)
+    ref = None
+    for junk in (0.0, math.nan, math.inf, 6e4):
+        x = [t.clone() for t in (q, k, v, dout)]
+        for b in range(3):
+            x[0][b, nq[b]:], x[3][b, nq[b]:] = junk, junk
+            x[1][b, nk[b]:], x[2][b, nk[b]:] = junk, junk
+        got = run(*x[:3], x[3], **how)
+        ref = ref or got
+        assert all(torch.equal(got[n], ref[n]) for n in got), junk
+    assert all(bool((ref[n][1] == 0).all()) for n in ref)
+
+
+def test_half_gradients_of_nothing_and_of_the_largest_and_smallest_values():
+    q, k, v, dout = inputs(2, 150, 150, 2, 2, 64, FP)
+    none = run(q, k, v, dout * 0)
+    assert all(bool((none[n] == 0).all()) for n in ("dq", "dk", "dv"))
+    # the largest half where the gradients fit all the same, the smallest where they are steps of 2^-24 themselves
+    check((q * 2**-12, k * 2**-12, v, dout.sign() * 65504), TWO_ROUNDINGS, names=("dq", "dk"))
+    check((q, k, v * 64, dout.sign() * 2**-24), TWO_ROUNDINGS)
+
+
+def test_half_gradients_in_two_graphs_that_are_replayed_in_turn():
+    x = [[t.to(DEV) for t in inputs(2, 330, 330, 4, 2, 64, FP, dout=s)] for s in (1e-4, 1e2)]
+
+    def make(q, k, v, _):
+        return [torch.empty_like(q), torch.empty(2, 4, 330, device=DEV), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)]
+
+    def go(x, b):
+        A.attention_fwd(*x[:3], b[0], b[1], dropout=0.1, seed=2)
+        A.attention_bwd(*x[:3], b[0], b[1], x[3], *b[2:], dropout=0.1, seed=2)
+
+    eager, bufs, graphs = [make(*y) for y in x], [make(*y) for y in x], [torch.cuda.CUDAGraph() for _ in x]
+    for y, b in zip(x, eager):
+        go(y, b)
+    torch.cuda.synchronize()
+    for y, b, graph in zip(x, bufs, graphs):
+        with torch.cuda.graph(graph):
+            go(y, b)
+    for _ in range(3):
+        for b in bufs:
+            for t in b:
+                t.zero_()
+        for graph in graphs:
+            graph.replay()
+        make(*x[0])
+        torch.cuda.synchronize()
+        for b, e in zip(bufs, eager):
+            assert all(torch.equal(s, t) for s, t in zip(b, e))

@@ -387,10 +387,12 @@ __device__ __forceinline__ unsigned step_of(const AttnArgs& a) {
 // ---------------------------------------------------------------------------------------------
 // Forward: one workgroup = 128 queries (4 waves x 32) of one head; tiles of 64 keys, double-
 // buffered in LDS.  grid = (sequence and head, tile): the tiles of a head land on one XCD, the
-// long ones are dispatched first.  Two sequences of 4096, 12 heads of 64: 80 us = 640 TFLOP/s of the
-// pairs seen; 32 x 1024 x 12 with dropout: 123 us.  Bound by the vector work on the probabilities
+// long ones are dispatched first.  Two sequences of 4096, 12 heads of 64: 82 us = 620 TFLOP/s of the
+// pairs seen; 32 x 1024 x 12 with dropout: 122 us.  P is rounded to the operands' type for the product (the
+// matrix unit takes no other), once, relative to a reference near the row's maximum; maximum, sum and O stay
+// in fp32: the output is 1.2 .. 1.4 times as far off as rounding it leaves.  Bound by the vector work on the probabilities
 // (an exponential, a maximum, a sum and a rounding each, half as much again with the mask) beside the
-// two products, at the clock that the power limit leaves (1.9 GHz).
+// two products, at the 1.9 GHz that the chip holds under it.
 //
 // KG = 2: a workgroup has 64 queries and two waves for each 32 of them, which take the even and the
 // odd tiles of keys and are joined through LDS at the end.  Twice as many workgroups of half the
@@ -579,7 +581,7 @@ attn_fwd_kernel(AttnArgs a) {
 // sequences, so a batch of short and long ones still fills the chip evenly.  What a chunk costs
 // apart from its keys (the first load, the joins) is worth some hundred keys, so there are no more
 // of them than workgroups run at once.  (Four caches of up to 8191 keys x 8 heads x 128, 84 MB:
-// 19.0 us + 5.4 us for the join with 512 workgroups, 4.4 TB/s; 23.0 + 4.9 with 256; without the
+// 18 .. 19 us + 5.1 us for the join with 512 workgroups, 4.4 .. 4.7 TB/s; 23.0 + 4.9 with 256; without the
 // hint that the keys are read once, which leaves the parts in L2, 20.2 + 6.2.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int kFewQueries = 32, kFewRows = 256, kFewTarget = 512;
@@ -888,7 +890,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int workgrou
 // per pair in fp32, is that error: dQ is corrected by -r (P K), at the cost of a fourth product,
 // and the dK / dV kernel that follows gets D + r.
 //
-// Both backward kernels on 32 x 1024 x 12 heads of 64 with dropout: 335 us (160 + 175), bound like
+// Both backward kernels on 32 x 1024 x 12 heads of 64 with dropout: 335 us (half: 351), bound like
 // the forward one; at 128 columns the accumulators leave one wave per SIMD (8 x 1024 x 16 heads:
 // 244 us), and a workgroup's time is 9 us + 1.2 us per 32 keys, which is what bounds ragged batches.
 //
@@ -1131,7 +1133,7 @@ attn_dq_kernel(AttnArgs a) {
 // that reads them.  Where that makes too few workgroups (few sequences, shared heads) the stages of
 // all heads are cut into ranges (key_plan), one workgroup each (blockIdx.z): they leave fp32 sums in
 // `parts` ([range][dK, dV][B][Hk][Tk][DP]) that attn_add_kernel adds in order.  (6 ragged sequences
-// of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 57 + 9 us in ranges.)
+// of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 57 + 9 us in ranges; now, with the exponents of half, 62 + 9.)
 template <class E, int DP, bool kDrop, bool kFine>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 && !kFine ? 2 : 1)))
 attn_dkdv_kernel(AttnArgs a) {

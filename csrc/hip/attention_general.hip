@@ -246,9 +246,9 @@ __device__ __forceinline__ void quad_transpose(unsigned (&w)[4], int lane) {
 
 // The factor of a query's dS: so that the largest one of the first tile with any lies in [2^6, 2^7), and
 // room for those that are up to 2^8 times larger; where a tile holds one beyond that, what was summed so far
-// is multiplied too.  (A narrower room costs: with a factor of 4 some of a wave's 32 rows pass it at every
-// sixth tile or so, and the dQ kernel of six sequences of up to 777 takes 58 us instead of 55; without any of this it takes 49.5,
-// the dK / dV kernel 61 instead of 63.)
+// is multiplied too.  (A narrower room costs: with a factor of 4 to 8 some of a wave's 32 rows pass it every
+// few tiles, and the dQ kernel of six sequences of up to 777, 16 heads on 4 of 128, takes 58 us instead of
+// 55.  Without any of this it takes 49.5, the dK / dV kernel 61 instead of 63.)
 struct GradScale {
     float x = 1.f, limit = 0.f, top = 0.f;  // |dS * x| up to `top` so far, `limit` allowed (0: all dS so far are 0)
 
@@ -390,8 +390,8 @@ __device__ __forceinline__ unsigned step_of(const AttnArgs& a) {
 // long ones are dispatched first.  Two sequences of 4096, 12 heads of 64: 82 us = 620 TFLOP/s of the
 // pairs seen; 32 x 1024 x 12 with dropout: 122 us.  P is rounded to the operands' type for the product (the
 // matrix unit takes no other), once, relative to a reference near the row's maximum; maximum, sum and O stay
-// in fp32: the output is 1.2 .. 1.4 times as far off as rounding it leaves.  Bound by the vector work on the probabilities
-// (an exponential, a maximum, a sum and a rounding each, half as much again with the mask) beside the
+// in fp32: the output is 1.2 .. 1.4 times as far off as rounding it leaves.  Bound by the vector work on
+// the probabilities (an exponential, a maximum, a sum and a rounding each, half as much again with the mask) beside the
 // two products, at the 1.9 GHz that the chip holds under it.
 //
 // KG = 2: a workgroup has 64 queries and two waves for each 32 of them, which take the even and the
@@ -1133,7 +1133,8 @@ attn_dq_kernel(AttnArgs a) {
 // that reads them.  Where that makes too few workgroups (few sequences, shared heads) the stages of
 // all heads are cut into ranges (key_plan), one workgroup each (blockIdx.z): they leave fp32 sums in
 // `parts` ([range][dK, dV][B][Hk][Tk][DP]) that attn_add_kernel adds in order.  (6 ragged sequences
-// of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 57 + 9 us in ranges; now, with the exponents of half, 62 + 9.)
+// of up to 777, 16 heads on 4 of 128: 145 us in 168 workgroups, 57 + 9 us in ranges; with the exponents of
+// half 63 + 9.)
 template <class E, int DP, bool kDrop, bool kFine>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 64 && !kFine ? 2 : 1)))
 attn_dkdv_kernel(AttnArgs a) {
